@@ -159,6 +159,21 @@ _SIGS = {
     "ar_hip_bpe_lookup": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, _c_int_p]),
     "ar_hip_bpe_encode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p,
                                          ctypes.c_int, _c_int_p]),
+    # include/ar_pages.h (the structures are common_amd.pages'; passed by reference)
+    "ar_hip_pages_work": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "ar_hip_pages_grow": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_size_t]),
+    "ar_hip_pages_trim": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int]),
+    "ar_hip_pages_fork": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]),
+    "ar_hip_pages_compact": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_size_t]),
+    "ar_hip_pages_copy": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int]),
+    "ar_hip_pages_write": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 4 +
+                           [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2 + [ctypes.c_float, ctypes.c_int] +
+                           [ctypes.c_void_p] * 2 + [ctypes.c_int]),
+    "ar_hip_attention_paged_work": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int,
+                                                                           ctypes.POINTER(ctypes.c_size_t)]),
+    "ar_hip_attention_paged": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                              ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                              ctypes.c_void_p, ctypes.c_size_t]),
 }
 
 

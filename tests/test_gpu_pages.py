@@ -1,0 +1,724 @@
+"""GPU checks of the paged cache (common_amd.pages, include/ar_pages.h) against numpy in 64 bits.
+
+Tolerances, per output value, u = 2^-24 (half a step of fp32) and r the half step of a 16-bit result (bf16 2^-8,
+fp16 2^-11):
+  attention: a score is a sum of head_dim products, off by at most 32 u S with S the largest sum of |q k| / sqrt(hd)
+      (sums in chains, whose errors add up as a random walk: sqrt(128) < 32); a weight is off by twice that relative
+      to itself and the sums over keys by 32 u again: (64 u S + 32 u) W with W = sum of weight |value|.  bf16
+      activations: queries are given in bf16, weights rounded to 16 bits add r W, the output's rounding r |out|.
+  write: norm, product and rotation in fp32: angles are exact to a double's rounding and then rounded to fp32 (2 u of
+      at most pi each for sin and cos, 4 u with their own error), 16 u of the head's largest value; storing adds r.
+Table calls and copies are exact.
+"""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+from common_amd import hardware as hw
+from common_amd import pages as pg
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF_STEP = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+CODE = {"f32": hw.DTYPE_F32, "f16": hw.DTYPE_F16, "bf16": hw.DTYPE_BF16}
+
+
+def _rng(seed):
+    return np.random.default_rng(seed)
+
+
+def _i32(ctx, values):
+    return ctx.to_device(np.asarray(values, np.int32))
+
+
+class Pool:
+    """A cache of random values with random tables, on the device and in numpy."""
+
+    def __init__(self, ctx, rng, dtype, layers, kv, hd, P, lengths, seqs=None, cols=None, spare=3, fill=None):
+        self.ctx, self.dtype, self.P = ctx, dtype, P
+        seqs = seqs or len(lengths)
+        need = [-(-n // P) for n in lengths]
+        cols = cols or max(need + [1])
+        pages = sum(need) + spare
+        order = rng.permutation(pages)
+        self.table = np.full((seqs, cols), -1, np.int32)
+        self.rows = np.zeros(seqs, np.int32)
+        for i, n in enumerate(need):
+            self.table[i, :n], order = order[:n], order[n:]
+            self.rows[i] = lengths[i]
+        self.refs = np.zeros(pages, np.int32)
+        self.refs[self.table[self.table >= 0]] = 1
+        shape = (layers, pages, kv, P, hd)
+        self.k, self.v = (ref.to_bits(rng.standard_normal(shape) if fill is None else np.full(shape, fill), dtype)
+                          for _ in range(2))
+        self.upload(layers, pages, kv, hd, seqs, cols)
+
+    def upload(self, layers, pages, kv, hd, seqs, cols):
+        b = {n: self.ctx.to_device(getattr(self, n)) for n in ("k", "v", "table", "rows", "refs")}
+        self.buf = b
+        self.cache = pg.PagedCache(self.ctx, layers, pages, kv, hd, seqs, cols, page_rows=self.P, dtype=CODE[self.dtype], **b)
+
+    def set(self, name, value):
+        setattr(self, name, value)
+        self.buf[name].upload(value)
+
+    def down(self, name):
+        a = getattr(self, name)
+        return self.buf[name].download(a.dtype, a.size).reshape(a.shape)
+
+    def free(self):
+        self.cache.close()
+        for b in self.buf.values():
+            b.free()
+
+    def seen(self, layer, seq):
+        """(keys, known), (values, known) of a sequence's whole table row, 64 bits."""
+        out = []
+        for pool in (self.k, self.v):
+            L, kv, hd = self.table.shape[1] * self.P, pool.shape[2], pool.shape[4]
+            x, known = np.zeros((L, kv, hd)), np.zeros(L, bool)
+            if 0 <= seq < len(self.table):
+                for c, page in enumerate(self.table[seq]):
+                    if 0 <= page < len(self.refs):
+                        x[c * self.P:(c + 1) * self.P] = ref.values(pool[layer, page]).transpose(1, 0, 2)
+                        known[c * self.P:(c + 1) * self.P] = True
+            out.append((x, known))
+        return out
+
+
+def _starts(counts):
+    return np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+
+
+def _attend(ctx, pool, layer, at, counts, q, act, heads, seq=None, extra=2, one_each=False):
+    """The call with `extra` rows behind the last chunk; returns [rows, heads, hd] float64 and checks those rows."""
+    total, hd = sum(counts), q.shape[2]
+    host = ref.to_bits(np.concatenate([q, np.full((extra, heads, hd), np.nan)]), act)
+    mark = np.full(host.shape, 0x4321 if act == "bf16" else 7.25, ref.STORED[act])
+    qd, od = ctx.to_device(host), ctx.to_device(mark)
+    bufs = [qd, od, _i32(ctx, at)] + ([] if one_each else [_i32(ctx, _starts(counts))])
+    sq = _i32(ctx, seq) if seq is not None else None
+    ch = pg.Chunks(len(counts), total + extra, at=bufs[2], start=None if one_each else bufs[3], seq=sq)
+    pool.cache.attention(layer, ch, qd, od, heads, CODE[act])
+    ctx.synchronize()
+    got = od.download(host.dtype, host.size).reshape(host.shape)
+    np.testing.assert_array_equal(got[total:], mark[total:])
+    for b in bufs + ([sq] if sq else []):
+        b.free()
+    return ref.values(got[:total])
+
+
+def _check_attention(got, pool, layer, at, counts, q, act, heads, seq=None):
+    starts = _starts(counts)
+    pairs = [pool.seen(layer, i if seq is None else seq[i]) for i in range(len(counts))]
+    qv = ref.values(ref.to_bits(q, act))
+    want = ref.attention([qv[starts[i]:starts[i + 1]] for i in range(len(counts))], [p[0] for p in pairs],
+                         [p[1] for p in pairs], at, counts, heads)
+    r = HALF_STEP[act]
+    for i, (out, mag, big) in enumerate(want):
+        g = got[starts[i]:starts[i + 1]]
+        tol = (64 * U * big + 32 * U + r) * mag + r * np.abs(out)
+        bad = ~(np.abs(g - out) <= tol)
+        assert not bad.any(), (i, np.argwhere(bad)[:4].tolist(), g[bad][:4], out[bad][:4], tol[bad][:4])
+
+
+TYPES = [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("bf16", "f32"), ("bf16", "f16"), ("bf16", "bf16")]
+
+
+@pytest.mark.parametrize("act,dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,hd,P", [(4, 2, 64, 16), (8, 8, 128, 32), (10, 2, 128, 64), (7, 1, 64, 128), (16, 2, 128, 256)])
+def test_attention_one_token_each(ctx, act, dtype, heads, kv, hd, P):
+    """Decode: one row of each sequence, contexts from none to several pages, ends inside a page and on its border."""
+    r = _rng(heads * hd + P)
+    at = [0, 1, P - 1, P, 2 * P - 1, 40, 63, 64, 65, 300, 1000]
+    pool = Pool(ctx, r, dtype, 2, kv, hd, P, [a + 1 for a in at])
+    q = r.standard_normal((len(at), heads, hd))
+    got = _attend(ctx, pool, 1, at, [1] * len(at), q, act, heads, one_each=True)
+    _check_attention(got, pool, 1, at, [1] * len(at), q, act, heads)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,hd,P,at,counts", [
+    (4, 2, 64, 16, [0, 5, 100], [1, 17, 33]),
+    (6, 2, 128, 32, [0, 31, 32, 200], [64, 0, 31, 3]),
+    (3, 3, 64, 64, [0], [130]),
+    (8, 1, 128, 16, [7, 250], [20, 5]),
+    (16, 8, 128, 64, [513], [129]),
+    (5, 1, 64, 256, [0, 700, 0], [0, 70, 260]),
+])
+def test_attention_chunks(ctx, act, dtype, heads, kv, hd, P, at, counts):
+    r = _rng(sum(at) + sum(counts) + hd)
+    pool = Pool(ctx, r, dtype, 1, kv, hd, P, [a + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), heads, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, act, heads)
+    _check_attention(got, pool, 0, at, counts, q, act, heads)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("scale", [1e-3, 8.0])
+def test_attention_flat_and_peaked_scores(ctx, act, dtype, scale):
+    """Scores next to zero (every key counts alike) and scores of tens (one key takes all)."""
+    r = _rng(3)
+    pool = Pool(ctx, r, dtype, 1, 2, 128, 32, [700, 260])
+    q = scale * r.standard_normal((41, 4, 128))
+    got = _attend(ctx, pool, 0, [699, 220], [1, 40], q, act, 4)
+    _check_attention(got, pool, 0, [699, 220], [1, 40], q, act, 4)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_split_long_context(ctx, act, dtype, hd):
+    """Few rows over long contexts (the keys are split over blocks), beside an empty and a short one."""
+    r = _rng(hd)
+    at, counts = [6000, 0, 9, 3333], [1, 1, 2, 5]
+    pool = Pool(ctx, r, dtype, 1, 2, hd, 64, [a + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), 4, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    _check_attention(got, pool, 0, at, counts, q, act, 4)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [70, 3, 40, 33]])
+def test_attention_of_rows_on_no_page(ctx, act, dtype, counts):
+    """Entries of -1 and outside the pool hide their rows; a sequence without any, an unknown one and a chunk that is
+    not in the cache see nothing and give zeros."""
+    r = _rng(11)
+    at = [500, 80, 130, -1]
+    pool = Pool(ctx, r, dtype, 1, 2, 64, 16, [571, 83, 170, 33])
+    t = pool.table.copy()
+    t[0, 3:9] = -1
+    t[0, 31] = len(pool.refs)
+    t[0, 32] = -2 ** 31
+    t[0, 33] = 2 ** 31 - 1
+    t[1] = -1
+    pool.set("table", t)
+    q = r.standard_normal((sum(counts), 4, 64))
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    _check_attention(got, pool, 0, at, counts, q, act, 4)
+    n = counts[0]
+    assert not got[n:n + counts[1]].any() and not got[n + counts[1] + counts[2]:].any()
+    seq = [2, 9, -1, 0]
+    got = _attend(ctx, pool, 0, [100, 5, 5, 400], counts, q, act, 4, seq=seq)
+    _check_attention(got, pool, 0, [100, 5, 5, 400], counts, q, act, 4, seq=seq)
+    pool.free()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("bf16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("hd,at,counts", [(64, [20, 60], [1, 1]), (128, [37, 5], [61, 9]), (64, [600, 90], [140, 3])])
+def test_hidden_rows_do_not_reach_the_result(ctx, bad, act, dtype, hd, at, counts):
+    """Rows behind the last one, free pages and, for a chunk's earlier rows, its later ones hold NaN or infinities."""
+    r = _rng(5)
+    pool = Pool(ctx, r, dtype, 1, 2, hd, 16, [a + c + 40 for a, c in zip(at, counts)])
+    hidden = ref.to_bits(np.full(1, bad), dtype)[0]
+    mid = [a + c // 2 for a, c in zip(at, counts)]  # rows from here on are spoilt; earlier queries must not notice
+    for i in range(len(at)):
+        for row in range(mid[i] + 1, int((pool.table[i] >= 0).sum()) * 16):
+            pool.k[0, pool.table[i, row // 16], :, row % 16] = hidden
+            pool.v[0, pool.table[i, row // 16], :, row % 16] = hidden
+    for page in np.flatnonzero(pool.refs == 0):
+        pool.k[0, page] = pool.v[0, page] = hidden
+    pool.set("k", pool.k)
+    pool.set("v", pool.v)
+    q = r.standard_normal((sum(counts), 4, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    starts = _starts(counts)
+    keep = np.concatenate([np.arange(starts[i], starts[i] + mid[i] - at[i] + 1) for i in range(len(at))])
+    short = [mid[i] - at[i] + 1 for i in range(len(at))]
+    _check_attention(got[keep], pool, 0, at, short, q[keep], act, 4)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_visible_infinity_reaches_only_who_sees_it(ctx, act, dtype, hd):
+    """A value of infinity in a chunk's row: later rows' results are infinite in that dim, earlier ones untouched, and
+    the other dims of all rows are what they were."""
+    r = _rng(17)
+    pool = Pool(ctx, r, dtype, 1, 1, hd, 16, [130])
+    q = r.standard_normal((90, 2, hd))
+    plain = _attend(ctx, pool, 0, [40], [90], q, act, 2)
+    v = pool.v.copy()
+    v[0, pool.table[0, 100 // 16], 0, 100 % 16, 9] = ref.to_bits(np.full(1, np.inf), dtype)[0]
+    pool.set("v", v)
+    got = _attend(ctx, pool, 0, [40], [90], q, act, 2)
+    assert np.isposinf(got[60:, :, 9]).all()
+    got[60:, :, 9] = plain[60:, :, 9]
+    np.testing.assert_array_equal(got, plain)
+    pool.free()
+
+
+def test_attention_with_chunk_starts_of_anything_stays_inside(ctx):
+    """Starts that descend or leave the rows make empty chunks; the proper ones among them are computed."""
+    r = _rng(23)
+    pool = Pool(ctx, r, "f16", 1, 2, 64, 16, [60, 60, 60, 60])
+    q = r.standard_normal((40, 4, 64))
+    for starts in ([0, 10, 5, 20, 40], [0, 10, 90, 95, 99], [-7, 3, 20, 2 ** 31 - 1, 9], [5, 5, 5, 5, 5]):
+        qd = ctx.to_device(q.astype(np.float32))
+        od = ctx.to_device(np.zeros((40, 4, 64), np.float32))
+        at, st = _i32(ctx, [20, 20, 20, 20]), _i32(ctx, starts)
+        pool.cache.attention(0, pg.Chunks(4, 40, at=at, start=st), qd, od, 4)
+        ctx.synchronize()
+        got = od.download(np.float32, q.size)
+        assert np.isfinite(got).all()
+        for b in (qd, od, at, st):
+            b.free()
+    pool.free()
+
+
+def test_attention_repeats_bit_for_bit(ctx):
+    r = _rng(29)
+    pool = Pool(ctx, r, "f16", 1, 2, 128, 64, [5000, 700])
+    q = r.standard_normal((8, 8, 128))
+    a = [_attend(ctx, pool, 0, [4999, 690], [1, 7], q, "f32", 8) for _ in range(4)]
+    for b in a[1:]:
+        np.testing.assert_array_equal(a[0], b)
+    pool.free()
+
+
+# ---- write -------------------------------------------------------------------------------------------
+
+SECTIONS = {1: (1,), 2: (5, 3), 3: (6, 5, 5), 4: (4, 4, 4, 4)}
+
+
+def _sections(half, axes):
+    s = [half * x // sum(SECTIONS[axes]) for x in SECTIONS[axes]]
+    s[0] += half - sum(s)
+    if axes == 3:
+        s = [half - 2 * (half // 3), half // 3, half // 3]
+    return s
+
+
+@pytest.mark.parametrize("act,dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,hd,P,axes,inter,mode,norm,stacked", [
+    (4, 2, 64, 16, 1, False, "head", True, True),
+    (6, 2, 128, 32, 3, False, "head", True, False),
+    (7, 7, 64, 64, 3, True, "whole", True, True),
+    (32, 8, 128, 16, 4, True, "head", True, True),
+    (40, 40, 64, 256, 2, False, "whole", True, False),
+    (5, 1, 128, 32, 2, True, "head", False, True),
+])
+def test_write(ctx, act, dtype, heads, kv, hd, P, axes, inter, mode, norm, stacked):
+    r = _rng(heads + hd + axes)
+    at, counts = [0, 15, 200, 31], [20, 1, 40, 0]
+    total, extra = sum(counts), 3
+    pool = Pool(ctx, r, dtype, 2, kv, hd, P, [a + c for a, c in zip(at, counts)])
+    before = pool.k.copy(), pool.v.copy()
+    q, k, v = (r.standard_normal((total + extra, n, hd)).astype(np.float32) for n in (heads, kv, kv))
+    gq = (1 + 0.1 * r.standard_normal((heads, hd))).astype(np.float32) if norm else None
+    gk = (1 + 0.1 * r.standard_normal((kv, hd))).astype(np.float32) if norm else None
+    pos = r.integers(0, 5000, (axes, total + extra)).astype(np.int32)
+    pos[:, 3] = 2 ** 31 - 1  # a far position
+    pos[0, 4] = -12
+    sec = _sections(hd // 2, axes)
+    bufs = []
+
+    def up(a):
+        bufs.append(ctx.to_device(a))
+        return bufs[-1]
+
+    if stacked:
+        qkv = up(np.concatenate([t.reshape(total + extra, -1) for t in (q, k, v)], 1))
+        qs = kvs = (heads + 2 * kv) * hd
+
+        class At:
+            def __init__(self, ptr):
+                self.ptr = ptr
+        qd, kd, vd = (At(qkv.ptr + 4 * hd * x) for x in (0, heads, heads + kv))
+    else:
+        qd, kd, vd = up(q), up(k), up(v)
+        qs = kvs = 0
+    mark = np.full((total + extra, heads, hd), 0x4321 if act == "bf16" else 7.25, ref.STORED[act])
+    out = up(mark)
+    ch = pg.Chunks(4, total + extra, at=up(np.array(at, np.int32)), start=up(_starts(counts)))
+    rot = pg.Rotary(1e6, up(pos), sec, pg.ROPE_INTERLEAVED if inter else pg.ROPE_SECTIONS)
+    pool.cache.write(1, ch, qd, kd, vd, out, heads, rot, CODE[act], qs, kvs, up(gq) if norm else None,
+                     up(gk) if norm else None, 1e-6, 1 if mode == "head" else 0)
+    ctx.synchronize()
+    got = out.download(mark.dtype, mark.size).reshape(mark.shape)
+    np.testing.assert_array_equal(got[total:], mark[total:])
+    axis = ref.rotary_axis(hd // 2, axes, sec, inter)
+    wq = ref.prepared(q[:total], gq, 1e-6, mode == "head", pos[:, :total], axis, 1e6)
+    wk = ref.prepared(k[:total], gk, 1e-6, mode == "head", pos[:, :total], axis, 1e6)
+
+    def close(a, b, t):
+        top = np.abs(b).max(-1, keepdims=True)
+        assert (np.abs(a - b) <= 16 * U * top + HALF_STEP[t] * (np.abs(b) + 16 * U * top) + 2.0 ** -24).all(), np.abs(a - b).max()
+
+    close(ref.values(got[:total]), wq, act)
+    kp, vp = pool.down("k"), pool.down("v")
+    starts = _starts(counts)
+    for i in range(4):
+        for j in range(counts[i]):
+            page, off = pool.table[i, (at[i] + j) // P], (at[i] + j) % P
+            close(ref.values(kp[1, page, :, off]), wk[starts[i] + j], dtype)
+            np.testing.assert_array_equal(vp[1, page, :, off], ref.to_bits(v[starts[i] + j], dtype))
+            kp[1, page, :, off], vp[1, page, :, off] = before[0][1, page, :, off], before[1][1, page, :, off]
+    np.testing.assert_array_equal(kp, before[0])  # nothing else changed
+    np.testing.assert_array_equal(vp, before[1])
+    pool.free()
+    for b in bufs:
+        b.free()
+
+
+def test_write_drops_rows_on_no_page_and_second_mentions(ctx):
+    """Keys and values of rows on no page, past the table, of unknown sequences, of chunks that are not in the cache
+    and of a sequence's second chunk are dropped; queries are prepared all the same; positions default to cache rows."""
+    r = _rng(31)
+    pool = Pool(ctx, r, "f32", 1, 1, 64, 16, [48, 48, 48])
+    t = pool.table.copy()
+    t[1, 1] = -1
+    t[2, 0] = len(pool.refs)
+    pool.set("table", t)
+    seq, at, counts = [1, 2, 0, 9, 1, 0], [14, 10, 40, 0, 0, -1], [5, 8, 20, 2, 6, 3]
+    n = sum(counts)
+    k, v, q = (r.standard_normal((n, h, 64)).astype(np.float32) for h in (1, 1, 2))
+    bufs = [ctx.to_device(x) for x in (q, k, v, np.zeros_like(q), np.array(at, np.int32), _starts(counts),
+                                       np.array(seq, np.int32))]
+    ch = pg.Chunks(6, n, at=bufs[4], start=bufs[5], seq=bufs[6])
+    pool.cache.write(0, ch, bufs[0], bufs[1], bufs[2], bufs[3], 2, pg.Rotary(1e4, None, [32]))
+    ctx.synchronize()
+    starts = _starts(counts)
+    want_k, want_v = pool.k.copy(), pool.v.copy()
+    pos = np.array([a + j if a >= 0 else 0 for a, c in zip(at, counts) for j in range(c)])[None]
+    axis = np.zeros(32, int)
+    pk, pq = ref.prepared(k, None, 0, True, pos, axis, 1e4), ref.prepared(q, None, 0, True, pos, axis, 1e4)
+    written = np.zeros(want_k.shape[:4], bool)
+    for i, (s, a, c) in enumerate(zip(seq, at, counts)):
+        for j in range(c):
+            if s in seq[:i] or not 0 <= s < 3 or a < 0 or a + j >= 48:
+                continue
+            page = t[s, (a + j) // 16]
+            if 0 <= page < len(pool.refs):
+                want_k[0, page, :, (a + j) % 16], want_v[0, page, :, (a + j) % 16] = pk[starts[i] + j], v[starts[i] + j]
+                written[0, page, :, (a + j) % 16] = True
+    assert written.sum() == 2 + 2 + 8  # rows 14, 15 of 1; 16, 17 of 2; 40..47 of 0
+    got_k = pool.down("k")
+    assert np.abs(got_k - want_k).max() <= 16 * U * np.abs(want_k).max()
+    np.testing.assert_array_equal(got_k[~written], pool.k[~written])
+    np.testing.assert_array_equal(pool.down("v"), want_v)
+    got_q = bufs[3].download(np.float32, q.size).reshape(q.shape)
+    assert np.abs(got_q - pq).max() <= 16 * U * np.abs(pq).max()
+    pool.free()
+    for b in bufs:
+        b.free()
+
+
+def test_write_in_place_and_without_queries(ctx):
+    r = _rng(37)
+    pool = Pool(ctx, r, "f16", 1, 2, 128, 32, [9, 9])
+    q, k, v = (r.standard_normal((18, h, 128)).astype(np.float32) for h in (4, 2, 2))
+    g = (1 + 0.1 * r.standard_normal((4, 128))).astype(np.float32)
+    qd, kd, vd, o, at, st, gd = (ctx.to_device(x) for x in (q, k, v, np.zeros_like(q), np.zeros(2, np.int32),
+                                                            np.array([0, 9, 18], np.int32), g))
+    ch, rot = pg.Chunks(2, 18, at=at, start=st), pg.Rotary(1e6, None, [64])
+    for mode in (0, 1):
+        qd.upload(q)
+        pool.cache.write(0, ch, qd, kd, vd, o, 4, rot, q_norm=gd, qk_norm_mode=mode)
+        k1, v1 = pool.down("k"), pool.down("v")
+        pool.set("k", pool.k)
+        pool.set("v", pool.v)
+        pool.cache.write(0, ch, None, kd, vd, None, 4, rot)
+        np.testing.assert_array_equal(pool.down("k"), k1)
+        np.testing.assert_array_equal(pool.down("v"), v1)
+        pool.cache.write(0, ch, qd, kd, vd, qd, 4, rot, q_norm=gd, qk_norm_mode=mode)
+        ctx.synchronize()
+        np.testing.assert_array_equal(qd.download(np.float32, q.size), o.download(np.float32, q.size))
+    pool.free()
+    for b in (qd, kd, vd, o, at, st, gd):
+        b.free()
+
+
+def test_write_rounds_past_fp16_to_infinity(ctx):
+    pool = Pool(ctx, _rng(1), "f16", 1, 1, 64, 16, [1])
+    k = np.zeros((1, 1, 64), np.float32)
+    k[0, 0, :3] = [65519.0, 65520.0, -70000.0]
+    kd, at = ctx.to_device(k), _i32(ctx, [0])
+    pool.cache.write(0, pg.Chunks(1, 1, at=at), None, kd, kd, None, 1, pg.Rotary(1e6, None, [32]))
+    got = pool.down("v")[0, pool.table[0, 0], 0, 0, :3]
+    np.testing.assert_array_equal(got, np.array([65504.0, np.inf, -np.inf], np.float16))
+    pool.free()
+    kd.free()
+    at.free()
+
+
+# ---- tables and pages ----------------------------------------------------------------------------------
+
+def _same(pool, t, copied=True):
+    for name in ("table", "rows", "refs"):
+        np.testing.assert_array_equal(pool.down(name), getattr(t, name), err_msg=name)
+    if copied:
+        k, v = pool.k.copy(), pool.v.copy()
+        for s, d in t.copied:
+            k[:, d], v[:, d] = pool.k[:, s], pool.v[:, s]
+        np.testing.assert_array_equal(pool.down("k"), k)
+        np.testing.assert_array_equal(pool.down("v"), v)
+        pool.k, pool.v = k, v
+    t.copied = []
+    pool.table, pool.rows, pool.refs = t.table.copy(), t.rows.copy(), t.refs.copy()
+
+
+def _grow(ctx, pool, t, counts, seq=None):
+    n = len(counts)
+    at, st, ms = _i32(ctx, [-5] * n), _i32(ctx, _starts(counts)), _i32(ctx, [-5])
+    sq = _i32(ctx, seq) if seq is not None else None
+    pool.cache.grow(pg.Chunks(n, sum(counts), at=at, start=st, seq=sq), ms)
+    want, missing = t.grow(range(n) if seq is None else seq, counts)
+    np.testing.assert_array_equal(at.download(np.int32, n), want)
+    assert ms.download(np.int32, 1)[0] == missing
+    for b in [at, st, ms] + ([sq] if sq else []):
+        b.free()
+    return want, missing
+
+
+def _trim(ctx, pool, t, seq, keep):
+    n = len(seq)
+    sq, kp = _i32(ctx, seq), _i32(ctx, keep) if keep is not None else None
+    pool.cache.trim(sq, kp, n)
+    t.trim(seq, keep)
+    ctx.synchronize()
+    sq.free()
+    if kp:
+        kp.free()
+
+
+def _fork(ctx, pool, t, src, dst):
+    a, b = _i32(ctx, src), _i32(ctx, dst)
+    pool.cache.fork(a, b, len(src))
+    t.fork(src, dst)
+    ctx.synchronize()
+    a.free()
+    b.free()
+
+
+def _tables(pool):
+    return ref.Tables(pool.table, pool.rows, pool.refs, pool.P)
+
+
+@pytest.mark.parametrize("dtype,kv,hd,P", [("f32", 2, 64, 16), ("bf16", 1, 128, 64), ("f16", 8, 128, 256)])
+def test_grow_fork_trim_step_by_step(ctx, dtype, kv, hd, P):
+    """Sequences share pages, grow apart, and are cut back; tables, counts and copied pages after every call."""
+    r = _rng(P)
+    pool = Pool(ctx, r, dtype, 2, kv, hd, P, [P + 3, 2 * P, 5, 0], seqs=9, cols=6, spare=14)
+    t = _tables(pool)
+    _fork(ctx, pool, t, [0, 0, 1, 2, 3], [4, 5, 6, 7, 8])
+    _same(pool, t)
+    _grow(ctx, pool, t, [1, 2, P, 0, P + 1, 1, 1, 2, 1])        # all sharers of one page in one call: the last keeps it
+    _same(pool, t)
+    _fork(ctx, pool, t, [4, 5], [5, 4])                          # sources that are targets
+    _same(pool, t)
+    _grow(ctx, pool, t, [3, 1], [5, 4])
+    _same(pool, t)
+    _trim(ctx, pool, t, [0, 4, 5, 8, 1], [P + 1, 2, -7, 0, 10 ** 9])
+    _same(pool, t)
+    _trim(ctx, pool, t, [6, 7, 6], None)
+    _same(pool, t)
+    assert (t.refs >= 0).all()
+    pool.free()
+
+
+def test_grow_without_enough_pages_or_columns(ctx):
+    r = _rng(2)
+    pool = Pool(ctx, r, "f32", 1, 1, 64, 16, [20, 20, 7, 30, 0], seqs=8, cols=4, spare=5)
+    t = _tables(pool)
+    _fork(ctx, pool, t, [0, 0], [5, 6])
+    _same(pool, t)
+    # 5 free pages; chunk 3 has no columns left, chunk 4 wants more than there is, 5 shares its page with 0 and 6
+    at, missing = _grow(ctx, pool, t, [10, 13, 2, 40, 64, 1, 1, 0])
+    assert missing > 0 and at[3] == -1 and at[4] == -1
+    _same(pool, t)
+    at, _ = _grow(ctx, pool, t, [1, 1, 1, 1, 1], [7, 7, -1, 8, 7])
+    assert at[0] == 0 and (at[1:] == -1).all()
+    _same(pool, t)
+    pool.free()
+
+
+def test_sharers_of_a_page_when_the_pool_runs_out(ctx):
+    """Three sequences on one last page and one free page: the first leaves it, the second cannot, so the third may
+    not write on it either."""
+    pool = Pool(ctx, _rng(4), "f32", 1, 1, 64, 16, [5], seqs=3, cols=2, spare=1)
+    t = _tables(pool)
+    _fork(ctx, pool, t, [0, 0], [1, 2])
+    at, missing = _grow(ctx, pool, t, [1, 1, 1])
+    assert at.tolist() == [5, -1, -1] and missing == 1
+    _same(pool, t)
+    at, missing = _grow(ctx, pool, t, [1, 1], [2, 0])
+    assert at.tolist() == [-1, 6] and missing == 1
+    _same(pool, t)
+    pool.free()
+
+
+def test_fork_passes_over_unknown_and_repeated_entries(ctx):
+    pool = Pool(ctx, _rng(6), "f32", 1, 1, 64, 16, [40, 17, 3], seqs=5, cols=3, spare=2)
+    t = _tables(pool)
+    _fork(ctx, pool, t, [0, 9, 1, -1, 2, 0, 1], [3, 4, 4, 1, 3, 7, 1])
+    _same(pool, t)
+    assert t.rows.tolist() == [40, 17, 3, 40, 17]
+    pool.free()
+
+
+@pytest.mark.parametrize("lengths,pages_spare", [([70, 3, 150, 0, 33], 9), ([16], 0), ([5], 1), ([16] * 40, 200)])
+def test_compact(ctx, lengths, pages_spare):
+    r = _rng(len(lengths))
+    pool = Pool(ctx, r, "bf16", 3, 2, 64, 16, lengths, cols=12, spare=pages_spare)
+    t = _tables(pool)
+    if len(lengths) > 2:
+        _fork(ctx, pool, t, [0], [1])
+        _same(pool, t)
+    live = _i32(ctx, [-1])
+    for _ in range(2):  # the second time nothing is left to move
+        pool.cache.compact(live)
+        ctx.synchronize()
+        want = t.compact()
+        assert live.download(np.int32, 1)[0] == want == (t.refs > 0).sum()
+        assert (t.refs[:want] > 0).all()
+        _same(pool, t)
+    live.free()
+    pool.free()
+
+
+def test_copy_between_pools(ctx):
+    r = _rng(8)
+    a = Pool(ctx, r, "f16", 3, 2, 128, 32, [320], spare=2)
+    b = Pool(ctx, r, "f16", 3, 2, 128, 32, [640], spare=1)
+    n, m = len(a.refs), len(b.refs)
+    src, dst = [0, 5, 5, n, 3, -1, 7, 2], [4, 9, 1, 2, 4, 8, m, m - 1]
+    sd, dd = _i32(ctx, src), _i32(ctx, dst)
+    a.cache.copy(b.cache, sd, dd, len(src))
+    ctx.synchronize()
+    k, v = b.k.copy(), b.v.copy()
+    for s, d in ((0, 4), (5, 9), (5, 1), (2, m - 1)):
+        k[:, d], v[:, d] = a.k[:, s], a.v[:, s]
+    np.testing.assert_array_equal(b.down("k"), k)
+    np.testing.assert_array_equal(b.down("v"), v)
+    np.testing.assert_array_equal(a.down("k"), a.k)
+    for x in (sd, dd):
+        x.free()
+    a.free()
+    b.free()
+
+
+def test_copy_within_a_pool(ctx):
+    pool = Pool(ctx, _rng(9), "f32", 2, 1, 64, 16, [160], spare=2)
+    src, dst = [0, 1, 2, 3, 3, 6], [7, 0, 8, 8, 9, 6]  # target 0 is a source, target 8 is named twice, 6 is its own
+    sd, dd = _i32(ctx, src), _i32(ctx, dst)
+    pool.cache.copy(pool.cache, sd, dd, len(src))
+    ctx.synchronize()
+    k, v = pool.k.copy(), pool.v.copy()
+    for s, d in ((0, 7), (2, 8), (3, 9)):
+        k[:, d], v[:, d] = pool.k[:, s], pool.v[:, s]
+    np.testing.assert_array_equal(pool.down("k"), k)
+    np.testing.assert_array_equal(pool.down("v"), v)
+    for x in (sd, dd):
+        x.free()
+    pool.free()
+
+
+def test_many_entries(ctx):
+    """As many chunks as a call takes, over a pool of more pages than one pass of its search covers."""
+    n = 4096
+    r = _rng(10)
+    lengths = r.integers(0, 20, n).tolist()
+    pool = Pool(ctx, r, "f32", 1, 1, 64, 16, lengths, cols=3, spare=2 * n)
+    t = _tables(pool)
+    _grow(ctx, pool, t, r.integers(0, 25, n).tolist(), r.permutation(n).tolist())
+    _same(pool, t)
+    _trim(ctx, pool, t, r.permutation(n).tolist(), r.integers(0, 30, n).tolist())
+    _same(pool, t)
+    pool.free()
+
+
+# ---- all of them together ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+def test_serving_loop_matches_whole_sequences(ctx, act, dtype):
+    """Prompts in chunks, a fork, single tokens and a rolled-back tail, with a compaction between: every row's
+    attention equals that over the sequence's own rows kept in plain arrays."""
+    r = _rng(77)
+    H, KV, hd, P, L, theta = 4, 2, 64, 16, 2, 1e6
+    cache = pg.PagedCache(ctx, L, 40, KV, hd, 4, 8, page_rows=P, dtype=CODE[dtype])
+    gq, gk = ((1 + 0.1 * r.standard_normal((n, hd))).astype(np.float32) for n in (H, KV))
+    gqd, gkd = ctx.to_device(gq), ctx.to_device(gk)
+    kept = [[(np.zeros((0, KV, hd)), np.zeros((0, KV, hd))) for _ in range(L)] for _ in range(4)]
+    axis = np.zeros(hd // 2, int)
+    ms = _i32(ctx, [0])
+    half = HALF_STEP[act]
+
+    def step(seqs, counts):
+        total = sum(counts)
+        at, st, sq = _i32(ctx, [-1] * len(seqs)), _i32(ctx, _starts(counts)), _i32(ctx, seqs)
+        ch = pg.Chunks(len(seqs), total, at=at, start=st, seq=sq)
+        cache.grow(ch, ms)
+        assert ms.download(np.int32, 1)[0] == 0
+        first = at.download(np.int32, len(seqs))
+        assert first.tolist() == [len(kept[s][0][0]) for s in seqs]
+        pos = np.concatenate([np.arange(a, a + c) for a, c in zip(first, counts)])[None]
+        for layer in range(L):
+            qkv = r.standard_normal((total, H + 2 * KV, hd)).astype(np.float32)
+            d = ctx.to_device(qkv)
+
+            class At:
+                def __init__(self, ptr):
+                    self.ptr = ptr
+            q, k, v = (At(d.ptr + 4 * hd * x) for x in (0, H, H + KV))
+            qo, o = (ctx.allocate(total * H * hd * 4) for _ in range(2))
+            w = (H + 2 * KV) * hd
+            cache.write(layer, ch, q, k, v, qo, H, pg.Rotary(theta, None, [hd // 2]), CODE[act], w, w, gqd, gkd, 1e-6, 1)
+            cache.attention(layer, ch, qo, o, H, CODE[act])
+            ctx.synchronize()
+            got = ref.values(o.download(ref.STORED[act], total * H * hd).reshape(total, H, hd))
+            # (from the queries as they were handed on, and the keys as the formula has them)
+            qv = ref.values(qo.download(ref.STORED[act], total * H * hd).reshape(total, H, hd))
+            pk = ref.prepared(qkv[:, H:H + KV], gk, 1e-6, True, pos, axis, theta)
+            starts = _starts(counts)
+            for i, s in enumerate(seqs):
+                a, b = starts[i], starts[i + 1]
+                kk = np.concatenate([kept[s][layer][0], ref.values(ref.to_bits(pk[a:b], dtype))])
+                vv = np.concatenate([kept[s][layer][1], ref.values(ref.to_bits(qkv[a:b, H + KV:], dtype))])
+                kept[s][layer] = (kk, vv)
+                known = np.ones(len(kk), bool)
+                (out, mag, big), = ref.attention([qv[a:b]], [(kk, known)], [(vv, known)], [first[i]], [b - a], H)
+                # a key next to the middle between two stored values may be rounded the other way: a whole step of S
+                step_k = 2 * HALF_STEP[dtype] / 8 if dtype != "f32" else 0
+                tol = (64 * U * big + 64 * U + half + step_k * big) * mag + half * np.abs(out)
+                assert (np.abs(got[a:b] - out) <= tol).all(), (s, layer, np.abs(got[a:b] - out).max())
+            for x in (d, qo, o):
+                x.free()
+        for x in (at, st, sq):
+            x.free()
+
+    def fork(s, d):
+        a, b = _i32(ctx, [s]), _i32(ctx, [d])
+        cache.fork(a, b, 1)
+        ctx.synchronize()
+        kept[d] = list(kept[s])
+        a.free()
+        b.free()
+
+    def trim(s, n):
+        a, b = _i32(ctx, [s]), _i32(ctx, [n])
+        cache.trim(a, b, 1)
+        ctx.synchronize()
+        kept[s] = [(k[:n], v[:n]) for k, v in kept[s]]
+        a.free()
+        b.free()
+
+    step([0, 1], [37, 5])
+    step([1, 0], [40, 1])
+    fork(0, 2)
+    step([0, 1, 2], [1, 1, 1])
+    step([2, 0], [20, 3])
+    trim(1, 0)
+    trim(0, 39)
+    cache.compact()
+    step([0, 1, 2], [1, 30, 1])
+    for _ in range(3):
+        step([2, 1, 0], [1, 1, 1])
+    ctx.synchronize()
+    cache.close()
+    for x in (gqd, gkd, ms):
+        x.free()
