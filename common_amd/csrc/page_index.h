@@ -25,14 +25,15 @@ AR_HD int cache_row(int at, int j) {
     return at + j;
 }
 
-// Chunks are cut into tiles of `span` rows.  Tile slots run over all chunks: chunk i has the slots from
-// chunk_slot(i) to chunk_slot(i + 1) - 1, which are enough for its tiles (a chunk of c rows from row s crosses at
-// most floor((s + c) / span) - floor(s / span) + 1 >= ceil(c / span) of them) and can be found without a prefix sum;
-// a slot past the chunk's last tile is empty.  All of them: at most rows / span + n.
-AR_HD int64_t chunk_slot(int32_t start, int i, int span) {
+// Chunks are cut into tiles of `span` units, `per_row` of them in a row (the query heads that share a KV head).  Tile
+// slots run over all chunks: chunk i has the slots from chunk_slot(i) to chunk_slot(i + 1) - 1, which are enough for its
+// tiles (c units from unit s on cross at most floor((s + c) / span) - floor(s / span) + 1 >= ceil(c / span) of them) and
+// can be found without a prefix sum; a slot past the chunk's last tile is empty.  All of them: at most
+// rows * per_row / span + n.
+AR_HD int64_t chunk_slot(int32_t start, int i, int per_row, int span) {
     // (floor also for negative starts: the slots of ascending starts ascend)
-    const int q = start >= 0 ? start / span : -((-(int64_t)start + span - 1) / span);
-    return (int64_t)q + i;
+    const int64_t s = (int64_t)start * per_row;
+    return (s >= 0 ? s / span : -((-s + span - 1) / span)) + i;
 }
 
 // Rows of chunk i as (first, count) within 0 .. rows; count 0 where start descends or leaves the range.
@@ -47,14 +48,19 @@ AR_HD void chunk_rows(const int32_t* start, int i, int rows, int* first, int* co
     *count = a >= 0 && b > a && b <= rows ? b - a : 0;
 }
 
-// The chunk that holds slot (or, with span 1, about row) `slot`: the last i with chunk_slot(start[i], i) <= slot.
-// For starts that ascend; for others some i in 0 .. n-1.
-AR_HD int chunk_of_slot(const int32_t* start, int n, int64_t slot, int span) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (chunk_slot(start[mid], mid, span) <= slot) lo = mid;
-        else hi = mid - 1;
+// The chunk that holds slot `slot`: the last i with chunk_slot(start[i], i) <= slot.  For starts that ascend; for others
+// some i in 0 .. n-1.  Each round asks `ways` chunks at once: `below(i, k, len)` tells how
+// many of the chunks i, i + k, i + 2k, ... below i + len satisfy the condition before the first that does not.
+template <typename F>
+AR_HD int chunk_search(int n, int ways, F below) {
+    int lo = 0, len = n;
+    while (len > 1) {
+        const int step = (len + ways - 1) / ways;
+        int c = below(lo, step, len);
+        if (c < 1) c = 1;
+        lo += (c - 1) * step;
+        len -= (c - 1) * step;
+        if (len > step) len = step;
     }
     return lo;
 }

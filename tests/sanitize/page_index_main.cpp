@@ -32,20 +32,28 @@ int main() {
             CHECK(chunk_of_row(start.data(), n, rows, r) == (r < 0 || r >= rows ? -1 : owner[r]));
         }
         // the slots: every tile of every chunk has one, in order, and their number is bounded
+        const int per = pick(1, 9);
+        auto of_slot = [&](int64_t slot) {
+            return chunk_search(n, 4, [&](int i, int k, int len) {
+                int c = 0;
+                for (int j = 0; j < 4 && j * k < len && chunk_slot(start[i + j * k], i + j * k, per, span) <= slot; j++) c++;
+                return c;
+            });
+        };
         int64_t before = 0;
         for (int i = 0; i < n; i++) {
-            const int64_t a = chunk_slot(start[i], i, span), b = chunk_slot(start[i + 1], i + 1, span);
-            CHECK(a == before && b - a >= (start[i + 1] - start[i] + span - 1) / span);
-            for (int64_t s = a; s < b; s++) CHECK(chunk_of_slot(start.data(), n, s, span) == i);
+            const int64_t a = chunk_slot(start[i], i, per, span), b = chunk_slot(start[i + 1], i + 1, per, span);
+            CHECK(a == before && b - a >= (per * (start[i + 1] - start[i]) + span - 1) / span);
+            for (int64_t s = a; s < b; s++) CHECK(of_slot(s) == i);
             before = b;
         }
-        CHECK(before <= rows / span + n);
+        CHECK(before <= (int64_t)rows * per / span + n);
         // one row each
         CHECK(chunk_of_row(nullptr, n, n + 3, n - 1) == n - 1 && chunk_of_row(nullptr, n, n + 3, n) == -1);
         // anything: indexes stay inside, counts stay inside the rows
         for (auto& s : start) s = any();
         for (int k = 0; k < 20; k++) {
-            const int c = chunk_of_row(start.data(), n, rows, any()), d = chunk_of_slot(start.data(), n, any(), span);
+            const int c = chunk_of_row(start.data(), n, rows, any()), d = of_slot(any());
             CHECK(c >= -1 && c < n && d >= 0 && d < n);
         }
         for (int i = 0; i < n; i++) {
