@@ -101,7 +101,7 @@ struct Shape {
     static constexpr int NQ = !QF ? 1 : F16 ? 2 : 3;      // planes of queries and of weights
     static constexpr int NK = !KF ? 1 : QF ? 3 : 2;       // planes of keys and values
     static constexpr int DEPTH = NQ > NK ? NQ : NK;       // plane pairs (i, j) with i + j < DEPTH are multiplied
-    static constexpr int BK = SMALL || KF ? 32 : 64;      // keys of a tile
+    static constexpr int BK = SMALL || KF || NQ == 3 ? 32 : 64;  // keys of a tile
     static constexpr int ROWS = SMALL ? 32 : 128;         // packed rows of a block
     static constexpr int NT = SMALL ? 64 : kThreads;      // threads that share a key tile
     static constexpr int CPR = HD / 8;                    // 8-value pieces of a row
@@ -281,7 +281,6 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
     const int t1 = min((split + 1) * t.per * step, (kend + BK - 1) / BK);
     const int* table = p.table + (size_t)(t.seq < 0 ? 0 : t.seq) * p.max_pages;
     const int pmask = (1 << p.shift) - 1;
-    constexpr int NPG = BK / 16;
 
     char* const kbuf = lds + (SMALL ? wave * C::TILE : 0);
     char* const vbuf = SMALL ? kbuf : lds + C::TILE;
@@ -293,36 +292,40 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
     const int vx = HD == 128 ? (vrow & 3) << 2 : ((vrow >> 1) & 1) << 2;
     const unsigned vaddr = vrow * (HD * 2) + (((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ vx) * 16) + (i16 & 1) * 8;
 
+    // A wavefront's 64 pieces of a load lie in 64 / CPR rows of one page (its first row is a multiple of that, and pages
+    // are longer), so that all but a fixed offset of each lane's address is the same for the wavefront.
+    constexpr int ROW = HD * (int)sizeof(KT);
     uint4 st[C::UNITS * (C::KF ? 2 : 1)];
-    int pg[NPG];
+    const unsigned lane_at = (lane / C::CPR) * ROW + (lane % C::CPR) * (8 * (int)sizeof(KT));
+    int pg0 = -1, pg1 = -1, pg2 = -1, pg3 = -1;
+    auto page_at = [&](int k0, int i) __attribute__((always_inline)) {
+        const int key = k0 + (i << p.shift);
+        int g = -1;
+        if ((i << p.shift) < BK && key < kend) g = table[key >> p.shift];
+        return g >= 0 && g < p.pages ? g : -1;
+    };
     auto load_pages = [&](int tile) __attribute__((always_inline)) {
         const int k0 = tile * BK;
-#pragma unroll
-        for (int i = 0; i < NPG; i++) {
-            pg[i] = -1;
-            const int key = k0 + (i << p.shift);
-            if ((i << p.shift) < BK && key < kend) {
-                const int g = table[key >> p.shift];
-                pg[i] = g >= 0 && g < p.pages ? g : -1;
-            }
+        pg0 = page_at(k0, 0);
+        pg1 = page_at(k0, 1);
+        if constexpr (BK > 32) {
+            pg2 = page_at(k0, 2);
+            pg3 = page_at(k0, 3);
         }
     };
+    // (a row on no page: some row of the pool in its place; keys are hidden by their scores, values zeroed below)
     auto stage_load = [&](int tile, const char* pool) __attribute__((always_inline)) {
-        const int k0 = tile * BK;
 #pragma unroll
         for (int u = 0; u < C::UNITS; u++) {
-            const int piece = u * C::NT + stid, key = piece / C::CPR, col = piece % C::CPR;
-            const int base = (u * C::NT + (SMALL ? 0 : wave * 64)) / C::CPR;  // the wavefront's first row: same page
-            int page = pg[0];
-#pragma unroll
-            for (int i = 1; i < NPG; i++) page = (base >> p.shift) == i ? pg[i] : page;
-            const char* src = pool + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((k0 + key) & pmask)) * (HD * sizeof(KT)) + col * 8 * sizeof(KT);
-            const bool in = page >= 0 && k0 + key < kend;
+            const int row0 = (u * C::NT + (SMALL ? 0 : wave * 64)) / C::CPR, i = row0 >> p.shift;
+            int page = i == 0 ? pg0 : i == 1 ? pg1 : i == 2 ? pg2 : pg3;
+            page = page < 0 ? 0 : page;
+            const char* src = pool + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((tile * BK + row0) & pmask)) * ROW;
             if constexpr (C::KF) {
-                st[2 * u] = in ? reinterpret_cast<const uint4*>(src)[0] : make_uint4(0, 0, 0, 0);
-                st[2 * u + 1] = in ? reinterpret_cast<const uint4*>(src)[1] : make_uint4(0, 0, 0, 0);
+                st[2 * u] = *reinterpret_cast<const uint4*>(src + lane_at);
+                st[2 * u + 1] = *reinterpret_cast<const uint4*>(src + lane_at + 16);
             } else {
-                st[u] = in ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+                st[u] = *reinterpret_cast<const uint4*>(src + lane_at);
             }
         }
     };
@@ -346,10 +349,18 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
             }
         }
     };
-    // Leaves infinities and NaN out of this thread's staged values; whether there were any.  A hidden key's weight of 0
-    // times one of them would reach rows that do not see it.
-    auto leave_out = [&]() __attribute__((always_inline)) {
+    // Zeros the staged values of rows on no page or behind the last key, and leaves infinities and NaN out of the others;
+    // whether there were any.  A hidden key's weight of 0 times one of them would reach rows that do not see it.
+    auto leave_out = [&](int k0, unsigned long long miss) __attribute__((always_inline)) {
         unsigned bad = 0;
+#pragma unroll
+        for (int u = 0; u < C::UNITS; u++) {
+            const int key = (u * C::NT + (SMALL ? 0 : wave * 64)) / C::CPR + lane / C::CPR;
+            if (k0 + key >= kend || (miss >> key & 1)) {
+                st[C::KF ? 2 * u : u] = make_uint4(0, 0, 0, 0);
+                if constexpr (C::KF) st[2 * u + 1] = make_uint4(0, 0, 0, 0);
+            }
+        }
         auto clean = [&](unsigned& w) __attribute__((always_inline)) {
             unsigned gone;
             if constexpr (C::KF) gone = (w & 0x7F800000u) == 0x7F800000u ? ~0u : 0u;
@@ -386,10 +397,11 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
     for (int tile = t0; tile < t1; tile += step) {
         const int k0 = tile * BK;
         unsigned long long miss = 0;  // keys of the tile that lie on no page
-#pragma unroll
-        for (int i = 0; i < NPG; i++)
-            if (pg[i] < 0 && (i << p.shift) < BK)
-                miss |= (p.shift >= 6 ? ~0ull : (1ull << (1 << p.shift)) - 1) << (i << p.shift & 63);
+        const unsigned long long page_keys = p.shift >= 6 ? ~0ull : (1ull << (1 << p.shift)) - 1;
+        if (pg0 < 0) miss |= page_keys;
+        if (pg1 < 0 && (1 << p.shift) < BK) miss |= page_keys << ((1 << p.shift) & 63);
+        if (pg2 < 0 && (2 << p.shift) < BK) miss |= page_keys << ((2 << p.shift) & 63);
+        if (pg3 < 0 && (3 << p.shift) < BK) miss |= page_keys << ((3 << p.shift) & 63);
         const bool masked = miss != 0 || k0 + BK - 1 > blim0;  // some row of the block does not see all of it
         stage_store(kbuf, false);
         stage_load(tile, p.vp);
@@ -414,14 +426,22 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                     }
                 }
             }
-            if (miss != 0 || k0 + BK - 1 > lim0) {
+            if (k0 + BK - 1 > lim0) {  // (the lane's keys are 32 kt + 8 (r / 4) + r % 4, and 4 h)
+                const int last = lim - k0 - 4 * h;
 #pragma unroll
                 for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int key = 32 * kt + 8 * (r >> 2) + 4 * h + (r & 3);
-                        if (k0 + key > lim || (miss >> key & 1)) s[kt][r] = -INFINITY;
-                    }
+                    for (int r = 0; r < 16; r++)
+                        if (32 * kt + 8 * (r >> 2) + (r & 3) > last) s[kt][r] = -INFINITY;
+            }
+            if (miss != 0) {
+#pragma unroll
+                for (int kt = 0; kt < KT32; kt++) {
+                    const unsigned gone = (unsigned)(miss >> (32 * kt)) >> (4 * h);
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (gone >> (8 * (r >> 2) + (r & 3)) & 1) s[kt][r] = -INFINITY;
+                }
             }
             float mx = s[0][0];
 #pragma unroll
@@ -453,7 +473,7 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
         }
         bool bad = false;
         if (masked) {
-            bad = leave_out();
+            bad = leave_out(k0, miss);
             if constexpr (SMALL) bad = __ballot(bad) != 0;
             else if (bad) s_bad = tile;
         }
@@ -467,6 +487,7 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
             for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
                 for (int k2 = 0; k2 < 2; k2++) {
+                    if (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // one step's planes at a time: registers
                     unsigned u[4][NQ];
 #pragma unroll
                     for (int i = 0; i < 4; i++) split2<C::F16, NQ>(s[kt][8 * k2 + 2 * i], s[kt][8 * k2 + 2 * i + 1], u[i]);
@@ -495,12 +516,14 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                     const int page = __builtin_amdgcn_readfirstlane(page_of_row(p.table, p.seqs, p.max_pages, p.pages, p.shift, t.seq, k0 + key));
                     if (page < 0) continue;
                     const KT* v = (const KT*)p.vp + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((k0 + key) & pmask)) * HD + 4 * h;
+                    const bool seen = k0 + key <= lim;
 #pragma unroll
                     for (int j = 0; j < NJ; j++)
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
                             const float x = to_float(v[32 * j + 8 * (r >> 2) + (r & 3)]);
-                            o[j][r] += k0 + key <= lim && !(fabsf(x) < INFINITY) ? x : 0.f;
+                            if (seen && !(fabsf(x) < INFINITY)) o[j][r] += x;
+                            if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // few loads at a time: registers
                         }
                 }
             }
