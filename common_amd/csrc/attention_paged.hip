@@ -19,9 +19,14 @@
 namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));  // (staged values stay in registers)
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ u32x4 quad(unsigned a, unsigned b, unsigned c, unsigned d) { return u32x4{a, b, c, d}; }
 
 struct PagedParams {
     const void* q;
@@ -30,9 +35,9 @@ struct PagedParams {
     const int *table, *seq, *start, *at;
     int heads, kv_heads, group, seqs, max_pages, pages, shift, n, rows;
     float scale;          // log2(e) / sqrt(head_dim)
-    int small_rows;       // chunks of at most this many packed rows are the few-row kernel's
-    int slots, splits;
-    float* part;          // [slots][kv_heads][splits][tile rows][hd] unnormalised outputs, then (m, l) of each
+    int few_rows;         // chunks of at most this many packed rows are the few-row kernel's
+    int tasks, target;    // tasks of the launch at most; how many to cut the keys for (0: whole rows)
+    float* part;          // [tasks][kv_heads][tile rows][hd] unnormalised outputs of splits, and (m, l) of each
     float2* part_ml;
 };
 
@@ -41,8 +46,11 @@ template <bool F16>
 struct Elem;
 template <>
 struct Elem<false> {
-    static __device__ __forceinline__ floatx16 mac(uint4 a, uint4 b, floatx16 c) {
+    static __device__ __forceinline__ floatx16 mac(u32x4 a, u32x4 b, floatx16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ floatx4 mac16(u32x4 a, u32x4 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     // two values rounded to nearest even, and what they stand for
     static __device__ __forceinline__ unsigned pack(float x, float y) {
@@ -56,8 +64,11 @@ struct Elem<false> {
 };
 template <>
 struct Elem<true> {
-    static __device__ __forceinline__ floatx16 mac(uint4 a, uint4 b, floatx16 c) {
+    static __device__ __forceinline__ floatx16 mac(u32x4 a, u32x4 b, floatx16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ floatx4 mac16(u32x4 a, u32x4 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ unsigned pack(float x, float y) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -82,6 +93,41 @@ __device__ __forceinline__ void split2(float x, float y, unsigned* out) {
     if constexpr (N > 2) out[2] = E::pack(x - E::low(out[1]), y - E::high(out[1]));
 }
 
+// fp32 products: a (bits) x b, 16 x 16 x 4
+__device__ __forceinline__ floatx4 mac4f(unsigned a, float b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mac4(unsigned a, unsigned b, floatx4 c) { return mac4f(a, __uint_as_float(b), c); }
+
+// Power of two that brings a row whose largest value is `top` into fp16's range, its largest to [2^14, 2^15).
+__device__ __forceinline__ int fp16_shift(float top) {
+    return top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 100) : 0;
+}
+
+// A piece of values (of fp32 or 16-bit ones) with zeros for infinities and NaN, which a hidden key's weight of 0 would
+// carry into rows that do not see them; *any becomes nonzero if there were some.
+template <bool KF, bool F16>
+__device__ __forceinline__ u32x4 drop_special(u32x4 v, unsigned* any) {
+    constexpr unsigned x = Elem<F16>::kExponent;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        unsigned gone;
+        if constexpr (KF) gone = (v[i] & 0x7F800000u) == 0x7F800000u ? ~0u : 0u;
+        else gone = ((v[i] & x) == x ? 0xFFFFu : 0u) | ((v[i] >> 16 & x) == x ? 0xFFFF0000u : 0u);
+        v[i] &= ~gone;
+        *any |= gone;
+    }
+    return v;
+}
+// The same for a piece in LDS, all of it where `out`.
+template <bool F16>
+__device__ __forceinline__ unsigned leave_out(u32x4* at, bool out) {
+    unsigned gone = 0;
+    const u32x4 v = drop_special<false, F16>(*at, &gone);
+    if (out || gone) *at = out ? quad(0, 0, 0, 0) : v;
+    return out ? 0u : gone;
+}
+
 template <typename T>
 struct Kind;
 template <>
@@ -93,78 +139,148 @@ struct Kind<_Float16> { static constexpr int id = AR_DTYPE_F16; };
 
 constexpr int kThreads = 256, kWaves = 4;
 
-// SMALL: a block takes 32 packed rows, and its wavefronts take key tiles in turn, each in an LDS space of its own.
-// Otherwise it takes 128 rows, 32 a wavefront, and the wavefronts share each key tile.
-template <int HD, typename QT, typename KT, bool SMALL>
+// Planes and sizes of a (head size, activation, cache) combination.
+template <int HD, typename QT, typename KT>
 struct Shape {
     static constexpr bool F16 = Kind<KT>::id == AR_DTYPE_F16, QF = Kind<QT>::id == AR_DTYPE_F32, KF = Kind<KT>::id == AR_DTYPE_F32;
     static constexpr int NQ = !QF ? 1 : F16 ? 2 : 3;      // planes of queries and of weights
     static constexpr int NK = !KF ? 1 : QF ? 3 : 2;       // planes of keys and values
     static constexpr int DEPTH = NQ > NK ? NQ : NK;       // plane pairs (i, j) with i + j < DEPTH are multiplied
-    static constexpr int BK = SMALL || KF || NQ == 3 ? 32 : 64;  // keys of a tile
-    static constexpr int ROWS = SMALL ? 32 : 128;         // packed rows of a block
-    static constexpr int NT = SMALL ? 64 : kThreads;      // threads that share a key tile
     static constexpr int CPR = HD / 8;                    // 8-value pieces of a row
-    static constexpr int UNITS = BK * CPR / NT;           // pieces of a tile per thread
+    // the tile kernel: 128 packed rows a block, 32 a wavefront, key tiles of BK shared by the block
+    static constexpr int ROWS = 128;
+    static constexpr int BK = KF || NQ == 3 ? 32 : 64;
+    static constexpr int UNITS = BK * CPR / kThreads;     // pieces of a tile per thread
     static constexpr int PLANE = BK * HD * 2;             // bytes of a plane of a tile
     static constexpr int TILE = NK * PLANE;
-    static constexpr int SETS = SMALL ? kWaves : 2;       // SMALL: a space per wavefront; else one for K, one for V
-    static constexpr int MERGE = SMALL ? 2 * 32 * HD * 4 : 0;  // two wavefronts' outputs
-    static constexpr int LDS = SETS * TILE > MERGE ? SETS * TILE : MERGE;
-    static constexpr int BLOCKS = SMALL && KF ? 1 : 2;   // of a CU, by registers and LDS
-    static constexpr float BIAS = F16 ? 14.f : 0.f;       // weights scaled by 2^14 in fp16: their small ones keep bits
+    static constexpr float BIAS = F16 ? 14.f : 0.f;  // weights scaled by 2^14 in fp16: their small ones keep bits
 };
 
-// What a block works on.
+// ---- what a block works on --------------------------------------------------------------------------------------
+// Tasks are the tiles of ROWS packed rows of every chunk, in the key splits of `per` units of kUnit keys.  Where there
+// are enough tiles to fill the GPU a task is a tile (p.target 0): the block's slot is searched among the chunks, 64 at a
+// time.  Otherwise every block adds up all chunks' units, so that `per` makes about p.target tasks of equal length
+// whatever the lengths of the sequences are, and finds its task in their order.
+constexpr int kUnit = 128;
+
 struct Task {
     int seq, first, count;  // chunk
     long long at;           // cache row of its first token
     int r0, rows;           // packed rows: first, and how many there are
-    int units, per, active; // key tiles in all, in a split, splits that have any
+    int units;              // key units its chunk's last row sees
+    int per, splits, split; // units of a split, splits, and which
+    int base;               // the tile's first task
 };
 
-// Slot, split -> task, by one wavefront (every wavefront of a block computes it for itself).
-template <int ROWS, int BKS>
-__device__ __forceinline__ bool find_task(const PagedParams& p, int slot, Task* t) {
+// Chunk i's rows, sequence and place; the number of its tiles (0: not this kernel's).
+template <int ROWS>
+__device__ __forceinline__ int chunk_tiles(const PagedParams& p, int i, Task* t) {
+    chunk_rows(p.start, i, p.rows, &t->first, &t->count);
+    const long long packed = (long long)t->count * p.group;
+    t->seq = p.seq ? p.seq[i] : i;
+    t->at = p.at[i];
+    const long long cap = (long long)p.max_pages << p.shift;
+    long long end = t->at + t->count;
+    if (end > cap) end = cap;
+    if (t->at < 0 || t->seq < 0 || t->seq >= p.seqs) end = 0;
+    t->units = (int)((end + kUnit - 1) / kUnit);
+    if (t->count == 0 || (ROWS == 16 ? packed > p.few_rows : packed <= p.few_rows)) return 0;
+    return (int)((packed + ROWS - 1) / ROWS);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// The table is read with scalar loads: nothing writes it while these kernels run.
+typedef const __attribute__((address_space(4))) int* TableRow;
+__device__ __forceinline__ TableRow table_row(const PagedParams& p, int seq) {
+    return (TableRow)(uintptr_t)(p.table + (size_t)(seq < 0 ? 0 : seq) * p.max_pages);
+}
+
+__device__ __forceinline__ long long wave_sum(long long v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Task `index` (MERGE: tile `index` of those with several splits or one) -> *t, by one wavefront; every wavefront of a
+// block computes it for itself.
+template <int ROWS, bool MERGE>
+__device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task* t) {
     const int lane = threadIdx.x & 63;
-    int chunk;
-    if (!p.start) {
-        const int tiles = (p.group + ROWS - 1) / ROWS;
-        chunk = slot / tiles;
-        t->r0 = (slot - chunk * tiles) * ROWS;
-    } else if (ROWS == 32 && p.small_rows == 32) {  // chunks of one tile: a slot each
-        chunk = slot;
-    } else {
-        chunk = chunk_search(p.n, 64, [&](int i, int k, int len) {
-            const bool below = (long long)lane * k < len && chunk_slot(p.start[i + lane * k], i + lane * k, p.group, ROWS) <= slot;
+    int tile;
+    if (p.target == 0) {
+        const int chunk = !p.start ? index / ((p.group + ROWS - 1) / ROWS) : chunk_search(p.n, 64, [&](int i, int k, int len) {
+            const bool below = (long long)lane * k < len && chunk_slot(p.start[i + lane * k], i + lane * k, p.group, ROWS) <= index;
             const unsigned long long m = __ballot(below);
             return m == ~0ull ? 64 : __builtin_ctzll(~m);
         });
-        chunk = __builtin_amdgcn_readfirstlane(chunk);
+        if (chunk >= p.n) return false;
+        const int tiles = chunk_tiles<ROWS>(p, chunk, t);
+        const long long at = !p.start ? index % ((p.group + ROWS - 1) / ROWS) : index - chunk_slot(t->first, chunk, p.group, ROWS);
+        if (at < 0 || at >= tiles) return false;
+        tile = (int)at;
+        t->per = t->units > 0 ? t->units : 1;
+        t->splits = 1;
+        t->split = 0;
+        t->base = index;
+    } else {
+        long long units = 0;
+        for (int i = lane; i < p.n; i += 64) {
+            Task c;
+            units += (long long)chunk_tiles<ROWS>(p, i, &c) * c.units;
+        }
+        units = wave_sum(units);
+        const int per = max(1, (int)((units + p.target - 1) / p.target));
+        long long tasks = 0, tiles = 0;  // before this round's chunks
+        bool found = false;
+        for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
+            Task c;
+            int n = 0, s = 1;
+            if (i0 + lane < p.n) {
+                n = chunk_tiles<ROWS>(p, i0 + lane, &c);
+                s = max(1, (c.units + per - 1) / per);
+            }
+            long long a = (long long)n * s, b = n;  // tasks and tiles up to and with this lane's chunk
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const long long x = __shfl_up(a, d), y = __shfl_up(b, d);
+                if (lane >= d) {
+                    a += x;
+                    b += y;
+                }
+            }
+            const unsigned long long m = __ballot((MERGE ? tiles + b : tasks + a) > index);
+            if (m) {
+                const int l = __builtin_ctzll(m);
+                const int chunk = i0 + l;
+                chunk_tiles<ROWS>(p, chunk, t);
+                n = __shfl(n, l);
+                t->splits = __shfl(s, l);
+                const long long a0 = tasks + __shfl(a, l) - (long long)n * t->splits, b0 = tiles + __shfl(b, l) - n;
+                const int at = (int)(index - (MERGE ? b0 : a0));
+                // (a tile's splits one after another)
+                tile = MERGE ? at : at / t->splits;
+                t->split = MERGE ? 0 : at - tile * t->splits;
+                t->base = (int)(a0 + (long long)tile * t->splits);
+                found = true;
+            }
+            tasks += __shfl(a, 63);
+            tiles += __shfl(b, 63);
+        }
+        if (!found) return false;
+        t->per = per;
     }
-    if (chunk >= p.n) return false;
-    chunk_rows(p.start, chunk, p.rows, &t->first, &t->count);
-    if (p.start) {
-        if (t->count == 0) return false;
-        const long long tile = ROWS == 32 && p.small_rows == 32 ? 0 : slot - chunk_slot(t->first, chunk, p.group, ROWS);
-        if (tile < 0 || tile * ROWS >= (long long)t->count * p.group) return false;
-        t->r0 = (int)(tile * ROWS);
-    }
-    const long long packed = (long long)t->count * p.group;
-    if (t->count == 0 || t->r0 >= packed) return false;
-    if (ROWS == 128 ? packed <= p.small_rows : packed > p.small_rows) return false;
-    t->rows = (int)(packed - t->r0 < ROWS ? packed - t->r0 : ROWS);
-    t->seq = p.seq ? p.seq[chunk] : chunk;
-    t->at = p.at[chunk];
-    // keys that the last row sees
-    const long long cap = (long long)p.max_pages << p.shift;
-    long long end = t->at + (t->r0 + t->rows - 1) / p.group + 1;
-    if (end > cap) end = cap;
-    if (t->at < 0 || t->seq < 0 || t->seq >= p.seqs) end = 0;
-    t->units = (int)((end + BKS - 1) / BKS);
-    t->per = (t->units + p.splits - 1) / p.splits;
-    if (t->per < 1) t->per = 1;
-    t->active = (t->units + t->per - 1) / t->per;
+    // (the same in every lane, and so in scalar registers)
+    t->seq = uniform(t->seq);
+    t->first = uniform(t->first);
+    t->count = uniform(t->count);
+    t->at = uniform((int)t->at);
+    t->units = uniform(t->units);
+    t->per = uniform(t->per);
+    t->splits = uniform(t->splits);
+    t->split = uniform(t->split);
+    t->base = uniform(t->base);
+    t->r0 = uniform(tile * ROWS);
+    t->rows = min(t->count * p.group - t->r0, ROWS);
     return true;
 }
 
@@ -177,13 +293,18 @@ __device__ __forceinline__ void load8<float>(const float* p, float* v) {
 }
 template <>
 __device__ __forceinline__ void load8<__hip_bfloat16>(const __hip_bfloat16* p, float* v) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
     const unsigned u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         v[2 * i] = __uint_as_float(u[i] << 16);
         v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
     }
+}
+__device__ __forceinline__ u32x4 load4(const float* p) { return *reinterpret_cast<const u32x4*>(p); }
+__device__ __forceinline__ u32x4 load4(const __hip_bfloat16* p) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    return quad(a.x << 16, a.x & 0xFFFF0000u, a.y << 16, a.y & 0xFFFF0000u);
 }
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
@@ -195,43 +316,35 @@ __device__ __forceinline__ void store4(__hip_bfloat16* p, float a, float b, floa
     *reinterpret_cast<uint2*>(p) = make_uint2(Elem<false>::pack(a, b), Elem<false>::pack(c, d));
 }
 
-template <int HD, typename QT, typename KT, bool SMALL>
-__global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void paged_tiles_kernel(PagedParams p) {
-    typedef Shape<HD, QT, KT, SMALL> C;
+template <int HD, typename QT, typename KT>
+__global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p) {
+    typedef Shape<HD, QT, KT> C;
     typedef Elem<C::F16> E;
     constexpr int NQ = C::NQ, NK = C::NK, BK = C::BK, KT32 = BK / 32, NJ = HD / 32, KS = HD / 16;
-    __shared__ __attribute__((aligned(16))) char lds[C::LDS];
-    __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+    __shared__ __attribute__((aligned(16))) char lds[2 * C::TILE];
     __shared__ int s_bad;
 
     const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // KV head fastest (8 of them: one to an XCD, whose L2 then holds that head's rows), later rows, with more keys, first
-    int b = blockIdx.x;
-    const int kvh = b % p.kv_heads;
-    b /= p.kv_heads;
-    const int split = b % p.splits, slot = p.slots - 1 - b / p.splits;
+    const int kvh = blockIdx.x % p.kv_heads;
     Task t;
-    if (!find_task<C::ROWS, SMALL ? 4 * BK : BK>(p, slot, &t)) return;
-    if (split >= (t.active > 0 ? t.active : 1)) return;
+    if (!find_task<C::ROWS, false>(p, p.tasks - 1 - (int)(blockIdx.x / p.kv_heads), &t)) return;
 
-    const int row = t.r0 + (SMALL ? 0 : 32 * wave) + lq, packed = t.r0 + t.rows;  // row: packed, in the chunk
+    const int row = t.r0 + 32 * wave + lq, packed = t.r0 + t.rows;  // row: packed, in the chunk
     const bool mine = row < packed;
     const int tok = mine ? row / p.group : 0, head = kvh * p.group + (mine ? row - tok * p.group : 0);
     const size_t qrow = ((size_t)(t.first + tok) * p.heads + head) * HD;
     const long long cap = (long long)p.max_pages << p.shift;
-    const bool present = t.units > 0;
-    // the last key a row sees; the block's and the wavefront's first and last rows'
-    const int lim = !mine || !present ? -1 : (int)(t.at + tok < cap ? t.at + tok : cap - 1);
-    const int w0 = t.r0 + (SMALL ? 0 : 32 * wave), w1 = (w0 + 31 < packed ? w0 + 31 : packed - 1);
-    const bool idle = w0 >= packed;
-    const int lim0 = idle || !present ? -1 : (int)(t.at + w0 / p.group < cap ? t.at + w0 / p.group : cap - 1);
-    const int lim1 = idle || !present ? -1 : (int)(t.at + w1 / p.group < cap ? t.at + w1 / p.group : cap - 1);
-    const int blim0 = !present ? -1 : (int)(t.at + t.r0 / p.group < cap ? t.at + t.r0 / p.group : cap - 1);
-    const int kend = !present ? 0 : (int)(t.at + (packed - 1) / p.group < cap ? t.at + (packed - 1) / p.group : cap - 1) + 1;
+    auto last_key = [&](int r) { return t.units == 0 ? -1 : (int)(t.at + r / p.group < cap ? t.at + r / p.group : cap - 1); };
+    // the last key a row sees; the wavefront's first and last rows', the block's
+    const int w0 = t.r0 + 32 * wave;
+    const int lim = mine ? last_key(row) : -1, lim0 = w0 < packed ? last_key(w0) : -1;
+    const int lim1 = w0 < packed ? last_key(min(w0 + 31, packed - 1)) : -1;
+    const int blim0 = last_key(t.r0), kend = last_key(packed - 1) + 1;
 
     // queries: planes in registers, rows of an fp16 cache's scaled into its range
-    uint4 qf[NQ][KS];
+    u32x4 qf[NQ][KS];
     float c = p.scale;
     {
         const QT* q = (const QT*)p.q + qrow;
@@ -250,8 +363,7 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[s][i]));
             top = max_xor32(top);
-            int e = 0;
-            if (top > 0.f && top < INFINITY) e = min(14 - ilogbf(top), 100);  // the largest in [2^14, 2^15)
+            const int e = fp16_shift(top);
             c = ldexpf(c, -e);
 #pragma unroll
             for (int s = 0; s < KS; s++)
@@ -264,7 +376,7 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
 #pragma unroll
             for (int i = 0; i < 4; i++) split2<C::F16, NQ>(v[s][2 * i], v[s][2 * i + 1], u[i]);
 #pragma unroll
-            for (int n = 0; n < NQ; n++) qf[n][s] = make_uint4(u[0][n], u[1][n], u[2][n], u[3][n]);
+            for (int n = 0; n < NQ; n++) qf[n][s] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
         }
     }
 
@@ -275,34 +387,29 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
         for (int r = 0; r < 16; r++) o[j][r] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    // key tiles of this split (SMALL: of this wavefront)
-    const int step = SMALL ? kWaves : 1;
-    const int t0 = SMALL ? split * t.per * kWaves + wave : split * t.per;
-    const int t1 = min((split + 1) * t.per * step, (kend + BK - 1) / BK);
-    const int* table = p.table + (size_t)(t.seq < 0 ? 0 : t.seq) * p.max_pages;
+    const int t0 = t.split * t.per * (kUnit / BK), t1 = min(t0 + t.per * (kUnit / BK), (kend + BK - 1) / BK);
+    const TableRow table = table_row(p, t.seq);
+    const int kmax = max(kend - 1, 0);
     const int pmask = (1 << p.shift) - 1;
 
-    char* const kbuf = lds + (SMALL ? wave * C::TILE : 0);
-    char* const vbuf = SMALL ? kbuf : lds + C::TILE;
-    const int stid = SMALL ? lane : tid;
+    char* const kbuf = lds;
+    char* const vbuf = lds + C::TILE;
     // swizzles of 16-byte pieces in a row: K, 16 rows of one column over all banks; V, 4 rows of 4 columns
     const int kx = HD == 128 ? lq & 15 : (lq >> 1) & 7;
     const unsigned kaddr = lq * (HD * 2) + ((h ^ kx) * 16);
     const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2);
-    const int vx = HD == 128 ? (vrow & 3) << 2 : ((vrow >> 1) & 1) << 2;
-    const unsigned vaddr = vrow * (HD * 2) + (((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ vx) * 16) + (i16 & 1) * 8;
+    auto value_swizzle = [](int key) { return HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; };
+    const unsigned vaddr = vrow * (HD * 2) + (((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ value_swizzle(vrow)) * 16) + (i16 & 1) * 8;
 
     // A wavefront's 64 pieces of a load lie in 64 / CPR rows of one page (its first row is a multiple of that, and pages
     // are longer), so that all but a fixed offset of each lane's address is the same for the wavefront.
     constexpr int ROW = HD * (int)sizeof(KT);
-    uint4 st[C::UNITS * (C::KF ? 2 : 1)];
+    u32x4 st[C::UNITS * (C::KF ? 2 : 1)];
     const unsigned lane_at = (lane / C::CPR) * ROW + (lane % C::CPR) * (8 * (int)sizeof(KT));
     int pg0 = -1, pg1 = -1, pg2 = -1, pg3 = -1;
     auto page_at = [&](int k0, int i) __attribute__((always_inline)) {
-        const int key = k0 + (i << p.shift);
-        int g = -1;
-        if ((i << p.shift) < BK && key < kend) g = table[key >> p.shift];
-        return g >= 0 && g < p.pages ? g : -1;
+        const int key = k0 + (i << p.shift), n = table[min(key, kmax) >> p.shift];
+        return (i << p.shift) < BK && key < kend && n >= 0 && n < p.pages ? n : -1;
     };
     auto load_pages = [&](int tile) __attribute__((always_inline)) {
         const int k0 = tile * BK;
@@ -314,87 +421,62 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
         }
     };
     // (a row on no page: some row of the pool in its place; keys are hidden by their scores, values zeroed below)
-    auto stage_load = [&](int tile, const char* pool) __attribute__((always_inline)) {
+    auto stage_load = [&](int tile, const char* pool, int a0, int a1, int a2, int a3) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < C::UNITS; u++) {
-            const int row0 = (u * C::NT + (SMALL ? 0 : wave * 64)) / C::CPR, i = row0 >> p.shift;
-            int page = i == 0 ? pg0 : i == 1 ? pg1 : i == 2 ? pg2 : pg3;
+            const int row0 = (u * kThreads + wave * 64) / C::CPR, i = row0 >> p.shift;
+            int page = i >= 1 ? a1 : a0;
+            page = i >= 2 ? a2 : page;
+            page = i >= 3 ? a3 : page;
             page = page < 0 ? 0 : page;
             const char* src = pool + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((tile * BK + row0) & pmask)) * ROW;
             if constexpr (C::KF) {
-                st[2 * u] = *reinterpret_cast<const uint4*>(src + lane_at);
-                st[2 * u + 1] = *reinterpret_cast<const uint4*>(src + lane_at + 16);
+                st[2 * u] = *reinterpret_cast<const u32x4*>(src + lane_at);
+                st[2 * u + 1] = *reinterpret_cast<const u32x4*>(src + lane_at + 16);
             } else {
-                st[u] = *reinterpret_cast<const uint4*>(src + lane_at);
+                st[u] = *reinterpret_cast<const u32x4*>(src + lane_at);
             }
         }
     };
     auto stage_store = [&](char* buf, bool values) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < C::UNITS; u++) {
-            const int piece = u * C::NT + stid, key = piece / C::CPR, col = piece % C::CPR;
-            const int x = values ? (HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2) : (HD == 128 ? key & 15 : (key >> 1) & 7);
+            const int piece = u * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
+            const int x = values ? value_swizzle(key) : HD == 128 ? key & 15 : (key >> 1) & 7;
             char* dst = buf + key * (HD * 2) + ((col ^ x) * 16);
             if constexpr (C::KF) {
-                const uint4 a = st[2 * u], d = st[2 * u + 1];
+                const u32x4 a = st[2 * u], d = st[2 * u + 1];
                 const unsigned w[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
                 unsigned pl[4][NK];
 #pragma unroll
                 for (int i = 0; i < 4; i++) split2<false, NK>(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), pl[i]);
 #pragma unroll
                 for (int n = 0; n < NK; n++)
-                    *reinterpret_cast<uint4*>(dst + n * C::PLANE) = make_uint4(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
+                    *reinterpret_cast<u32x4*>(dst + n * C::PLANE) = quad(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
             } else {
-                *reinterpret_cast<uint4*>(dst) = st[u];
+                *reinterpret_cast<u32x4*>(dst) = st[u];
             }
         }
     };
-    // Zeros the staged values of rows on no page or behind the last key, and leaves infinities and NaN out of the others;
-    // whether there were any.  A hidden key's weight of 0 times one of them would reach rows that do not see it.
-    auto leave_out = [&](int k0, unsigned long long miss) __attribute__((always_inline)) {
-        unsigned bad = 0;
-#pragma unroll
-        for (int u = 0; u < C::UNITS; u++) {
-            const int key = (u * C::NT + (SMALL ? 0 : wave * 64)) / C::CPR + lane / C::CPR;
-            if (k0 + key >= kend || (miss >> key & 1)) {
-                st[C::KF ? 2 * u : u] = make_uint4(0, 0, 0, 0);
-                if constexpr (C::KF) st[2 * u + 1] = make_uint4(0, 0, 0, 0);
-            }
+    // Zeros this thread's pieces of values that are not there, infinities and NaN, in LDS; whether there were any of
+    // these.  (Few tiles need it: a loop, and in LDS, for the sake of the others' registers.)
+    auto clean = [&](int k0, unsigned long long miss) __attribute__((always_inline)) {
+        unsigned any = 0;
+#pragma unroll 1
+        for (int u = 0; u < C::UNITS * NK; u++) {
+            const int piece = u / NK * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
+            u32x4* const at = reinterpret_cast<u32x4*>(vbuf + u % NK * C::PLANE + key * (HD * 2) + ((col ^ value_swizzle(key)) * 16));
+            any |= leave_out<C::F16>(at, k0 + key >= kend || (miss >> key & 1));
         }
-        auto clean = [&](unsigned& w) __attribute__((always_inline)) {
-            unsigned gone;
-            if constexpr (C::KF) gone = (w & 0x7F800000u) == 0x7F800000u ? ~0u : 0u;
-            else gone = ((w & E::kExponent) == E::kExponent ? 0xFFFFu : 0u) | ((w >> 16 & E::kExponent) == E::kExponent ? 0xFFFF0000u : 0u);
-            w &= ~gone;
-            bad |= gone;
-        };
-#pragma unroll
-        for (int u = 0; u < C::UNITS * (C::KF ? 2 : 1); u++) {
-            clean(st[u].x);
-            clean(st[u].y);
-            clean(st[u].z);
-            clean(st[u].w);
-        }
-        return bad != 0;
-    };
-    auto tile_sync = [&]() __attribute__((always_inline)) {
-        if constexpr (SMALL) {
-            // one wavefront's own LDS space: its accesses are served in order
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_wave_barrier();
-        } else {
-            __syncthreads();
-        }
+        return any != 0;
     };
 
-    if constexpr (!SMALL) {
-        if (tid == 0) s_bad = -1;
-    }
+    if (tid == 0) s_bad = -1;
     if (t0 < t1) {
         load_pages(t0);
-        stage_load(t0, p.kp);
+        stage_load(t0, p.kp, pg0, pg1, pg2, pg3);
     }
-    for (int tile = t0; tile < t1; tile += step) {
+    for (int tile = t0; tile < t1; tile++) {
         const int k0 = tile * BK;
         unsigned long long miss = 0;  // keys of the tile that lie on no page
         const unsigned long long page_keys = p.shift >= 6 ? ~0ull : (1ull << (1 << p.shift)) - 1;
@@ -404,9 +486,9 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
         if (pg3 < 0 && (3 << p.shift) < BK) miss |= page_keys << ((3 << p.shift) & 63);
         const bool masked = miss != 0 || k0 + BK - 1 > blim0;  // some row of the block does not see all of it
         stage_store(kbuf, false);
-        stage_load(tile, p.vp);
-        load_pages(tile + step);  // (past the split's end: not used)
-        tile_sync();
+        stage_load(tile, p.vp, pg0, pg1, pg2, pg3);
+        load_pages(tile + 1);  // (past the split's end: not used)
+        __syncthreads();
 
         const bool work = k0 <= lim1;
         floatx16 s[KT32];
@@ -419,7 +501,7 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                 for (int ks = 0; ks < KS; ks++) {
 #pragma unroll
                     for (int j = 0; j < NK; j++) {
-                        const uint4 kf = *reinterpret_cast<const uint4*>(kbuf + j * C::PLANE + kt * 32 * HD * 2 + (kaddr ^ (ks * 32)));
+                        const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + j * C::PLANE + kt * 32 * HD * 2 + (kaddr ^ (ks * 32)));
 #pragma unroll
                         for (int i = 0; i < NQ; i++)
                             if (i + j < C::DEPTH) s[kt] = E::mac(kf, qf[i][ks], s[kt]);
@@ -471,17 +553,11 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                 }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);  // this lane's half of the keys
         }
-        bool bad = false;
-        if (masked) {
-            bad = leave_out(k0, miss);
-            if constexpr (SMALL) bad = __ballot(bad) != 0;
-            else if (bad) s_bad = tile;
-        }
         stage_store(vbuf, true);
-        const int next = tile + step;
-        if (next < t1) stage_load(next, p.kp);
-        tile_sync();
-        if constexpr (!SMALL) bad = masked && s_bad == tile;
+        if (masked && clean(k0, miss)) s_bad = tile;
+        if (tile + 1 < t1) stage_load(tile + 1, p.kp, pg0, pg1, pg2, pg3);
+        __syncthreads();
+        const bool bad = masked && s_bad == tile;
         if (work) {
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
@@ -491,9 +567,9 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                     unsigned u[4][NQ];
 #pragma unroll
                     for (int i = 0; i < 4; i++) split2<C::F16, NQ>(s[kt][8 * k2 + 2 * i], s[kt][8 * k2 + 2 * i + 1], u[i]);
-                    uint4 pf[NQ];
+                    u32x4 pf[NQ];
 #pragma unroll
-                    for (int n = 0; n < NQ; n++) pf[n] = make_uint4(u[0][n], u[1][n], u[2][n], u[3][n]);
+                    for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
 #pragma unroll
                     for (int jt = 0; jt < NJ; jt++)
 #pragma unroll
@@ -502,8 +578,8 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                             typedef __attribute__((address_space(3))) shortx4 lds4;
                             const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a);
                             const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(a + 8 * HD * 2));
-                            const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
-                            const uint4 vf = make_uint4(x.x, x.y, y.x, y.y);
+                            const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+                            const u32x4 vf = quad(x.x, x.y, y.x, y.y);
 #pragma unroll
                             for (int i = 0; i < NQ; i++)
                                 if (i + j < C::DEPTH) o[jt] = E::mac(vf, pf[i], o[jt]);
@@ -528,45 +604,11 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
                 }
             }
         }
-        if constexpr (SMALL) tile_sync();
     }
     l = sum_xor32(l);
 
-    if constexpr (SMALL) {  // the wavefronts' states: a common maximum, then the sums of 2 + 3 into 0 + 1, of 1 into 0
-        if (h == 0) s_m[wave][lq] = m;
-        __syncthreads();
-        float mm = s_m[0][lq];
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) mm = fmaxf(mm, s_m[w][lq]);
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
-        l *= f;
-        m = mm;
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[j][r] *= f;
-        if (h == 0) s_l[wave][lq] = l;
-        float* const mine_o = reinterpret_cast<float*>(lds) + lane;
-#pragma unroll
-        for (int half = 2; half > 0; half /= 2) {
-            __syncthreads();
-            if (wave >= half && wave < 2 * half)
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) mine_o[(((wave - half) * NJ + j) * 16 + r) * 64] = o[j][r];
-            __syncthreads();
-            if (wave < half)
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[j][r] += mine_o[((wave * NJ + j) * 16 + r) * 64];
-        }
-        if (wave > 0) return;
-        l = (s_l[0][lq] + s_l[1][lq]) + (s_l[2][lq] + s_l[3][lq]);
-    }
     if (!mine) return;
-    if (t.active <= 1) {
+    if (t.splits == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         QT* out = (QT*)p.out + qrow;
 #pragma unroll
@@ -575,7 +617,7 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
             for (int r = 0; r < 16; r += 4)
                 store4(out + 32 * j + 2 * r + 4 * h, o[j][r] * inv, o[j][r + 1] * inv, o[j][r + 2] * inv, o[j][r + 3] * inv);
     } else {
-        const size_t at = (((size_t)slot * p.kv_heads + kvh) * p.splits + split) * C::ROWS + (row - t.r0);
+        const size_t at = ((size_t)(t.base + t.split) * p.kv_heads + kvh) * C::ROWS + (row - t.r0);
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
@@ -585,116 +627,450 @@ __global__ __launch_bounds__(kThreads, (Shape<HD, QT, KT, SMALL>::BLOCKS)) void 
     }
 }
 
-// The splits of a row, in their order.  A block takes four rows of a task.
-template <int HD, typename QT, int ROWS, int BKS>
-__global__ __launch_bounds__(4 * HD) void paged_merge_kernel(PagedParams p) {
+// ---- few rows: one token of a sequence, or some ----------------------------------------------------------------------
+// A block takes 16 packed rows and its four wavefronts take key tiles of 32 in turn, so that a decode step streams its
+// keys and values from as many places as there are wavefronts, with no barrier between them.  16 x 16 matrix
+// instructions: S^T (16 keys x 16 rows) twice, lane l has row l % 16 and keys 4 (l / 16) + 0..3; O^T (16 dims x 16 rows)
+// from 32 keys at a time.  Keys go from memory straight into the operands (a lane's 16 bytes lie beside its three
+// neighbours' in the row).  16-bit values take the way over the wavefront's own LDS space, for the transposed reads;
+// fp32 ones do not: v_mfma_f32_16x16x4_f32 wants one value of a key per lane, and output row i of tile (a, j) is dim
+// 64 a + 4 i + j, so that 16 bytes of a value row feed four tiles.  Of the next tile, keys are loaded when this one's
+// scores are done and values when its own are in LDS (or used).
+template <int HD, typename QT, typename KT>
+__global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
+    typedef Shape<HD, QT, KT> C;
+    typedef Elem<C::F16> E;
+    constexpr bool KF = C::KF;
+    constexpr int NQ = C::NQ, NJ = HD / 16, KS = HD / 32, QC = HD / 16, JJ = HD / 64;
+    constexpr int ROW = HD * (int)sizeof(KT), UNITS = 32 * C::CPR / 64, VBYTES = 32 * HD * 2;
+    __shared__ __attribute__((aligned(16))) char lds[kWaves * VBYTES];  // values, later the wavefronts' outputs
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+
+    const int tid = threadIdx.x, lane = tid & 63, lq = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.x % p.kv_heads;
+    Task t;
+    if (!find_task<16, false>(p, blockIdx.x / p.kv_heads, &t)) return;
+    const int row = t.r0 + lq, packed = t.r0 + t.rows;
+    const bool mine = row < packed;
+    const int tok = mine ? row / p.group : 0, head = kvh * p.group + (mine ? row - tok * p.group : 0);
+    const size_t qrow = ((size_t)(t.first + tok) * p.heads + head) * HD;
+    const long long cap = (long long)p.max_pages << p.shift;
+    auto last_key = [&](int r) { return t.units == 0 ? -1 : (int)(t.at + r / p.group < cap ? t.at + r / p.group : cap - 1); };
+    const int lim = mine ? last_key(row) : -1, lim0 = last_key(t.r0), kend = last_key(packed - 1) + 1;
+    const int t0 = t.split * t.per * 4 + wave, t1 = min((t.split + 1) * t.per * 4, (kend + 31) / 32);
+
+    const TableRow table = table_row(p, t.seq);
+    const int kmax = max(kend - 1, 0);
+    const int pmask = (1 << p.shift) - 1;
+    auto page_at = [&](int tile, int i) __attribute__((always_inline)) {  // page of the tile's keys 16 i on
+        const int key = 32 * tile + 16 * i, n = table[min(key, kmax) >> p.shift];
+        return key < kend && n >= 0 && n < p.pages ? n : -1;
+    };
+    // start of the pool row of key 16 i of a tile (a row on no page: some row of the pool in its place)
+    auto row_at = [&](const char* pool, int tile, int page, int key) __attribute__((always_inline)) {
+        return pool + ((((size_t)(page < 0 ? 0 : page) * p.kv_heads + kvh) << p.shift) + ((32 * tile + key) & pmask)) * ROW;
+    };
+    u32x4 kf[2][KF ? QC : KS], vf[KF ? 2 * 4 * JJ : UNITS];
+    const unsigned k_at = lq * ROW + g * 16;
+    const unsigned v_at = KF ? 4 * g * ROW + lq * 16 : (lane / C::CPR) * ROW + (lane % C::CPR) * 16;
+    int pg0 = page_at(t0, 0), pg1 = page_at(t0, 1);
+    auto load_k = [&](int tile, int a0, int a1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const char* src = row_at(p.kp, tile, a ? a1 : a0, 16 * a) + k_at;
+#pragma unroll
+            for (int s = 0; s < (KF ? QC : KS); s++) kf[a][s] = *reinterpret_cast<const u32x4*>(src + 64 * s);
+        }
+    };
+    auto load_v = [&](int tile, int a0, int a1) __attribute__((always_inline)) {
+        if constexpr (KF) {
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                const char* src = row_at(p.vp, tile, a ? a1 : a0, 16 * a) + v_at;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int j = 0; j < JJ; j++) vf[(4 * a + r) * JJ + j] = *reinterpret_cast<const u32x4*>(src + r * ROW + 256 * j);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < UNITS; u++) {
+                const int key = u * 64 / C::CPR;
+                vf[u] = *reinterpret_cast<const u32x4*>(row_at(p.vp, tile, key >= 16 ? a1 : a0, key) + v_at);
+            }
+        }
+    };
+    if (t0 < t1) {
+        load_k(t0, pg0, pg1);
+        load_v(t0, pg0, pg1);
+    }
+    int pn0 = page_at(t0 + kWaves, 0), pn1 = page_at(t0 + kWaves, 1);
+
+    // queries
+    u32x4 qf[KF ? 1 : NQ][KF ? QC : KS];
+    float c = p.scale;
+    if constexpr (KF) {
+#pragma unroll
+        for (int s = 0; s < QC; s++) qf[0][s] = mine ? load4((const QT*)p.q + qrow + 16 * s + 4 * g) : quad(0, 0, 0, 0);
+    } else {
+        float v[KS][8];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            if (mine) load8<QT>((const QT*)p.q + qrow + 32 * s + 8 * g, v[s]);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[s][i] = 0.f;
+        }
+        if constexpr (C::F16) {
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[s][i]));
+            top = max_xor32(fmaxf(top, xor16(top, lane)));
+            const int e = fp16_shift(top);
+            c = ldexpf(c, -e);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[s][i] = ldexpf(v[s][i], e);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            unsigned u[4][NQ];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split2<C::F16, NQ>(v[s][2 * i], v[s][2 * i + 1], u[i]);
+#pragma unroll
+            for (int n = 0; n < NQ; n++) qf[n][s] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
+        }
+    }
+
+    floatx4 o[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) o[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    // values in LDS: swizzled so that 8 rows of two 16-byte pieces lie over all banks (transposed reads)
+    char* const vbuf = lds + wave * VBYTES;
+    auto swizzle = [](int key) { return HD == 128 ? (key & 3) << 2 | (key >> 2 & 1) << 1 : (key >> 1 & 3) << 1; };
+    const int vrow = 4 * g + (lq >> 2);
+    const unsigned vaddr = vrow * (HD * 2) + ((((lq & 3) >> 1) ^ swizzle(vrow)) * 16) + (lq & 1) * 8;
+
+    for (int tile = t0; tile < t1; tile += kWaves) {
+        const int k0 = 32 * tile;
+        const unsigned miss = (pg0 < 0 ? 0xFFFFu : 0u) | (pg1 < 0 ? 0xFFFF0000u : 0u);  // keys on no page (or past the end)
+        const bool masked = miss != 0 || k0 + 31 > lim0;
+        floatx4 s[2];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            s[a] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (KF) {
+                floatx4 s1 = s[a];
+#pragma unroll
+                for (int q = 0; q < QC; q++) {
+                    floatx4& x = q & 1 ? s1 : s[a];
+                    x = mac4(kf[a][q].x, qf[0][q].x, x);
+                    x = mac4(kf[a][q].y, qf[0][q].y, x);
+                    x = mac4(kf[a][q].z, qf[0][q].z, x);
+                    x = mac4(kf[a][q].w, qf[0][q].w, x);
+                }
+                s[a] += s1;
+            } else {
+#pragma unroll
+                for (int q = 0; q < KS; q++)
+#pragma unroll
+                    for (int i = 0; i < NQ; i++) s[a] = E::mac16(kf[a][q], qf[i][q], s[a]);
+            }
+        }
+        const int next = tile + kWaves;
+        load_k(next, pn0, pn1);  // (past the end: rows of no page, not used)
+        if (masked) {
+            const int last = lim - k0 - 4 * g;
+            const unsigned gone = miss >> (4 * g);
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (16 * a + r > last || (gone >> (16 * a + r) & 1)) s[a][r] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = max_xor32(fmaxf(mx, xor16(mx, lane))) * c;
+        if (__ballot(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) o[j] *= alpha;
+            m = mn;
+        }
+        const float mu = m == -INFINITY ? 0.f : m - C::BIAS;  // (no key seen yet: weights 0)
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[a][r] = __builtin_amdgcn_exp2f(fmaf(s[a][r], c, -mu));
+        l += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+        // (as in the tile kernel: values of rows that are not there, infinities and NaN are left out)
+        bool bad = false;
+        if constexpr (KF) {
+            if (masked) {
+                unsigned any = 0;
+#pragma unroll
+                for (int u = 0; u < 2 * 4 * JJ; u++) {
+                    const int key = 16 * (u / (4 * JJ)) + 4 * g + u / JJ % 4;
+                    if (k0 + key >= kend || (miss >> key & 1)) vf[u] = quad(0, 0, 0, 0);
+                    vf[u] = drop_special<true, false>(vf[u], &any);
+                    __builtin_amdgcn_sched_barrier(0);  // one piece at a time: registers
+                }
+                bad = __ballot(any != 0) != 0;
+            }
+        }
+        if constexpr (KF) {
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int j = 0; j < JJ; j++) {
+                        const u32x4 v = vf[(4 * a + r) * JJ + j];
+                        o[4 * j] = mac4f(v.x, s[a][r], o[4 * j]);
+                        o[4 * j + 1] = mac4f(v.y, s[a][r], o[4 * j + 1]);
+                        o[4 * j + 2] = mac4f(v.z, s[a][r], o[4 * j + 2]);
+                        o[4 * j + 3] = mac4f(v.w, s[a][r], o[4 * j + 3]);
+                    }
+            load_v(next, pn0, pn1);
+        } else {
+#pragma unroll
+            for (int u = 0; u < UNITS; u++) {
+                const int key = u * 64 / C::CPR + lane / C::CPR, col = lane % C::CPR;
+                *reinterpret_cast<u32x4*>(vbuf + key * (HD * 2) + ((col ^ swizzle(key)) * 16)) = vf[u];
+            }
+            load_v(next, pn0, pn1);
+            if (masked) {
+                unsigned any = 0;
+#pragma unroll 1
+                for (int u = 0; u < UNITS; u++) {
+                    const int key = u * 64 / C::CPR + lane / C::CPR, col = lane % C::CPR;
+                    any |= leave_out<C::F16>(reinterpret_cast<u32x4*>(vbuf + key * (HD * 2) + ((col ^ swizzle(key)) * 16)),
+                                             k0 + key >= kend || (miss >> key & 1));
+                }
+                bad = __ballot(any != 0) != 0;
+            }
+            asm volatile("" ::: "memory");  // (one wavefront's LDS accesses are served in order)
+            __builtin_amdgcn_wave_barrier();
+            u32x4 pf[NQ];
+            {
+                unsigned u[4][NQ];
+#pragma unroll
+                for (int i = 0; i < 4; i++) split2<C::F16, NQ>(s[i >> 1][2 * (i & 1)], s[i >> 1][2 * (i & 1) + 1], u[i]);
+#pragma unroll
+                for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                typedef __attribute__((address_space(3))) shortx4 lds4;
+                const char* a = vbuf + (vaddr ^ (j * 32));
+                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a));
+                const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(a + 16 * HD * 2)));
+#pragma unroll
+                for (int i = 0; i < NQ; i++) o[j] = E::mac16(quad(x.x, x.y, y.x, y.y), pf[i], o[j]);
+            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (__builtin_expect(bad, 0)) {
+#pragma unroll 1
+            for (int key = 0; key < 32 && k0 + key < kend; key++) {
+                const int page = key >= 16 ? pg1 : pg0;
+                if (page < 0) continue;
+                const KT* v = (const KT*)row_at(p.vp, tile, page, key);
+                const bool seen = k0 + key <= lim;
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float x = to_float(v[KF ? 64 * (j / 4) + 4 * (4 * g + r) + j % 4 : 16 * j + 4 * g + r]);
+                        if (seen && !(fabsf(x) < INFINITY)) o[j][r] += x;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        pg0 = pn0;
+        pg1 = pn1;
+        pn0 = page_at(next + kWaves, 0);
+        pn1 = page_at(next + kWaves, 1);
+    }
+
+    // the wavefronts' states at a common maximum; each adds up a quarter of the outputs
+    l += xor16(l, lane);
+    l = sum_xor32(l);
+    if (g == 0) s_m[wave][lq] = m;
+    __syncthreads();  // (values in LDS are done with, too)
+    float mm = s_m[0][lq];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) mm = fmaxf(mm, s_m[w][lq]);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+    if (g == 0) s_l[wave][lq] = l * f;
+    float* const st = reinterpret_cast<float*>(lds) + lane;  // [wavefront][tile][register][lane]
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) st[((wave * NJ + j) * 4 + r) * 64] = o[j][r] * f;
+    __syncthreads();
+    if (!mine) return;
+    l = (s_l[0][lq] + s_l[1][lq]) + (s_l[2][lq] + s_l[3][lq]);
+    const size_t at = ((size_t)(t.base + t.split) * p.kv_heads + kvh) * 16 + lq;
+    const float inv = t.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int q = 0; q < NJ / 4; q++) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // 16-bit caches: tile q + NJ / 4 * wave, register i; fp32: tiles 4 q + i, register `wave`
+            const float* a = st + (KF ? (4 * q + i) * 4 + wave : (q + NJ / 4 * wave) * 4 + i) * 64;
+            v[i] = ((a[0] + a[NJ * 256]) + (a[2 * NJ * 256] + a[3 * NJ * 256])) * inv;
+        }
+        const int d = KF ? 64 * q + 4 * (4 * g + wave) : 16 * (q + NJ / 4 * wave) + 4 * g;
+        if (t.splits > 1) store4(p.part + at * HD + d, v[0], v[1], v[2], v[3]);
+        else store4((QT*)p.out + qrow + d, v[0], v[1], v[2], v[3]);
+    }
+    if (t.splits > 1 && wave == 0 && g == 0) p.part_ml[at] = make_float2(mm, l);
+}
+
+// ---- the splits of a row, in a fixed order ------------------------------------------------------------------------
+// A block takes 16 rows of a tile; where a tile has fewer, several groups of HD / 4 lanes share a row's splits.
+template <int HD, typename QT, int ROWS>
+__global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
+    constexpr int LPR = HD / 4, NG = 512 / LPR;
+    __shared__ __attribute__((aligned(16))) float s_o[NG][HD];
+    __shared__ float s_l[NG];
     int b = blockIdx.x;
     const int kvh = b % p.kv_heads;
     b /= p.kv_heads;
-    const int quad = b % (ROWS / 4), slot = b / (ROWS / 4);
+    const int r0 = 16 * (b % (ROWS / 16));
     Task t;
-    if (!find_task<ROWS, BKS>(p, slot, &t) || t.active <= 1) return;
-    const int r = 4 * quad + threadIdx.x / HD, d = threadIdx.x % HD;
-    if (r >= t.rows) return;
-    const size_t at = (((size_t)slot * p.kv_heads + kvh) * p.splits) * ROWS + r;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int s = 0; s < t.active; s++) m = fmaxf(m, p.part_ml[at + (size_t)s * ROWS].x);
-    for (int s = 0; s < t.active; s++) {
-        const float2 ml = p.part_ml[at + (size_t)s * ROWS];
-        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+    if (!find_task<ROWS, true>(p, b / (ROWS / 16), &t) || t.splits == 1) return;
+    const int rows = min(t.rows - r0, 16);
+    if (rows <= 0) return;
+    int share = 1;  // groups of a row
+    while (2 * share * rows <= NG) share *= 2;
+    const int group = threadIdx.x / LPR, col = threadIdx.x % LPR, r = group / share, sub = group % share;
+    const size_t step = (size_t)p.kv_heads * ROWS, at = ((size_t)t.base * p.kv_heads + kvh) * ROWS + r0 + min(r, rows - 1);
+    float m = -INFINITY, l = 0.f;
+    for (int s = col; s < t.splits; s += LPR) m = fmaxf(m, p.part_ml[at + s * step].x);
+#pragma unroll
+    for (int d = 1; d < LPR; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = sub; s < t.splits; s += share) {
+        const float2 ml = p.part_ml[at + s * step];
+        const float4 v = *reinterpret_cast<const float4*>(p.part + (at + s * step) * HD + 4 * col);
+        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // (no key seen: zeros)
         l = fmaf(ml.y, f, l);
-        // (a split without a visible key holds zeros)
-        o = fmaf(p.part[(at + (size_t)s * ROWS) * HD + d], f, o);
+        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
     }
-    const int row = t.r0 + r, tok = row / p.group, head = kvh * p.group + row - tok * p.group;
-    const float v = l == 0.f ? 0.f : o / l;
-    QT* out = (QT*)p.out + ((size_t)(t.first + tok) * p.heads + head) * HD + d;
-    if constexpr (sizeof(QT) == 4) *reinterpret_cast<float*>(out) = v;
-    else *reinterpret_cast<uint16_t*>(out) = (uint16_t)bf16_rne_bits(v);
+    *reinterpret_cast<float4*>(&s_o[group][4 * col]) = o;
+    if (col == 0) s_l[group] = l;
+    __syncthreads();
+    if (sub != 0 || r >= rows) return;
+    for (int k = 1; k < share; k++) {
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[group + k][4 * col]);
+        o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+        l += s_l[group + k];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int row = t.r0 + r0 + r, tok = row / p.group, head = kvh * p.group + row - tok * p.group;
+    store4((QT*)p.out + ((size_t)(t.first + tok) * p.heads + head) * HD + 4 * col, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
 
-// The launches of a call.  Chunks of few packed rows go to the few-row kernel, which splits a chunk's keys over the
-// wavefronts of a block too; where the call's rows are few for its chunks, all of them do.
-struct Plan {
-    bool small = false, big = false;
-    int small_rows = 0;                 // the few-row kernel's chunks
-    int small_slots = 0, small_splits = 1, big_slots = 0, big_splits = 1;
-    size_t bytes = 16;
+// A kernel's share of a call: tasks at most, and how many to cut the keys for (0: none).
+struct Part {
+    int tiles = 0, target = 0;
+    int tasks() const { return tiles + target; }
+    size_t bytes(const ar_pages* p, int rows) const {
+        return target ? (size_t)tasks() * p->kv_heads * rows * ((size_t)p->head_dim * 4 + 8) : 0;
+    }
 };
 
-size_t part_bytes(const ar_pages* p, int slots, int splits, int rows) {
-    return splits <= 1 ? 0 : (size_t)slots * p->kv_heads * splits * rows * ((size_t)p->head_dim * 4 + 8);
-}
+// The launches of a call.  The host knows the numbers of rows and of chunks, not which chunk has how many: where the
+// rows are few for the chunks every chunk goes to the few-row kernel, where there is one chunk of many rows it goes to
+// the tile kernel, otherwise both are launched and share the chunks by their rows.
+struct Plan {
+    int few_rows = 0;  // packed rows up to which a chunk is the few-row kernel's
+    Part few, tile;
+};
 
-int splits_for(const ar_pages* p, int slots, int per_cu, int cus, int keys) {
-    const long long cap = (long long)p->max_pages * p->page_rows, most = (cap + keys - 1) / keys;
-    const long long want = ((long long)per_cu * cus + (long long)slots * p->kv_heads - 1) / ((long long)slots * p->kv_heads);
-    return (int)std::max(1LL, std::min(std::min(want, most), 64LL));
+constexpr int kFewRows = 64, kMaxSplitChunks = 1024;
+
+// Tasks to cut the keys for: `per_cu` blocks a CU over all KV heads, unless the tiles alone are several times that.
+int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu) {
+    if (tiles * p->kv_heads >= 3LL * per_cu * ctx->num_cus || n > kMaxSplitChunks) return 0;
+    if ((long long)p->max_pages * p->page_rows <= kUnit) return 0;
+    return std::max(1, per_cu * ctx->num_cus / p->kv_heads);
 }
 
 int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int heads, Plan* out) {
     const long long group = heads / p->kv_heads, packed = (long long)c->rows * group;
+    AR_CHECK_ARG(packed <= 1 << 30 && (packed / 16 + c->n) * p->kv_heads <= 1 << 30, "paged attention: %d rows of %d heads are too many",
+                 c->rows, heads);
     Plan a;
-    AR_CHECK_ARG(packed <= 1 << 30, "paged attention: %d rows of %lld heads per KV head are too many", c->rows, group);
+    const int few_cu = p->dtype == AR_DTYPE_F32 ? 2 : 3;
     if (!c->start || packed <= 32LL * c->n) {
-        a.small = true;
-        a.small_rows = 0x7fffffff;
-        const long long slots = !c->start ? (long long)c->n * ((group + 31) / 32) : packed / 32 + c->n;
-        AR_CHECK_ARG(slots * p->kv_heads <= 0x7fffffffLL / 64, "paged attention: %d rows of %d heads are too many", c->rows,
-                     heads);
-        a.small_slots = (int)slots;
+        a.few_rows = 0x7fffffff;
+        a.few.tiles = (int)(c->start ? packed / 16 + c->n : c->n * ((group + 15) / 16));
+        a.few.target = target_of(ctx, p, std::max<long long>(c->n, packed / 16), c->n, few_cu);
     } else {
-        a.big = true;
-        const long long slots = packed / 128 + c->n;
-        AR_CHECK_ARG(slots * p->kv_heads <= 0x7fffffffLL / 64, "paged attention: %d rows of %d heads are too many", c->rows,
-                     heads);
-        a.big_slots = (int)slots;
+        a.tile.tiles = (int)(packed / 128 + c->n);
+        a.tile.target = target_of(ctx, p, packed / 128, c->n, 2);
         if (c->n > 1) {
-            a.small = true;
-            a.small_rows = 32;
-            a.small_slots = c->n;
+            a.few_rows = kFewRows;
+            a.few.target = target_of(ctx, p, 0, c->n, few_cu);
+            a.few.tiles = (int)(a.few.target ? std::min(packed / 16 + c->n, kFewRows / 16LL * c->n) : packed / 16 + c->n);
         }
     }
-    if (a.small) a.small_splits = splits_for(p, std::min(a.small_slots, c->n * (int)((group + 31) / 32)), 2, ctx->num_cus, 128);
-    if (a.big) a.big_splits = splits_for(p, a.big_slots, 2, ctx->num_cus, 128);
-    a.bytes = std::max<size_t>(16, part_bytes(p, a.small_slots, a.small_splits, 32) + part_bytes(p, a.big_slots, a.big_splits, 128));
     *out = a;
     return AR_HIP_OK;
 }
 
-template <int HD, typename QT, typename KT, bool SMALL>
-int launch_tiles(PagedParams p, int slots, int splits, char* work, hipStream_t st) {
-    typedef Shape<HD, QT, KT, SMALL> C;
-    p.slots = slots;
-    p.splits = splits;
-    const size_t rows = (size_t)slots * p.kv_heads * splits * C::ROWS;
-    p.part = (float*)work;
-    p.part_ml = (float2*)(work + rows * HD * 4);
-    hipLaunchKernelGGL((paged_tiles_kernel<HD, QT, KT, SMALL>), dim3((unsigned)((long long)slots * p.kv_heads * splits)),
-                       dim3(kThreads), 0, st, p);
-    AR_LAUNCH_CHECK();
-    if (splits > 1) {
-        hipLaunchKernelGGL((paged_merge_kernel<HD, QT, C::ROWS, SMALL ? 4 * C::BK : C::BK>),
-                           dim3((unsigned)((long long)slots * p.kv_heads * (C::ROWS / 4))), dim3(4 * HD), 0, st, p);
+size_t plan_bytes(const ar_pages* p, const Plan& a) { return std::max<size_t>(16, a.few.bytes(p, 16) + a.tile.bytes(p, 128)); }
+
+template <int HD, typename QT, typename KT>
+int launch_plan(const ar_pages* pages, const Plan& a, PagedParams p, char* work, hipStream_t st) {
+    auto part = [&](const Part& x, int rows, char* at) {
+        p.tasks = x.tasks();
+        p.target = x.target;
+        p.part = (float*)at;
+        p.part_ml = (float2*)(at + (size_t)x.tasks() * p.kv_heads * rows * HD * 4);
+    };
+    if (a.tile.tiles) {
+        part(a.tile, 128, work + a.few.bytes(pages, 16));
+        hipLaunchKernelGGL((paged_tiles_kernel<HD, QT, KT>), dim3((unsigned)p.tasks * p.kv_heads), dim3(kThreads), 0, st, p);
         AR_LAUNCH_CHECK();
+        if (p.target) {
+            hipLaunchKernelGGL((paged_merge_kernel<HD, QT, 128>), dim3((unsigned)a.tile.tiles * 8 * p.kv_heads), dim3(512), 0, st, p);
+            AR_LAUNCH_CHECK();
+        }
+    }
+    if (a.few.tiles) {
+        part(a.few, 16, work);
+        hipLaunchKernelGGL((paged_few_kernel<HD, QT, KT>), dim3((unsigned)p.tasks * p.kv_heads), dim3(kThreads), 0, st, p);
+        AR_LAUNCH_CHECK();
+        if (p.target) {
+            hipLaunchKernelGGL((paged_merge_kernel<HD, QT, 16>), dim3((unsigned)a.few.tiles * p.kv_heads), dim3(512), 0, st, p);
+            AR_LAUNCH_CHECK();
+        }
     }
     return AR_HIP_OK;
 }
 
-template <int HD, typename QT, typename KT>
-int launch_plan(const Plan& a, const PagedParams& p, char* work, size_t big_at, hipStream_t st) {
-    if (a.big) AR_TRY((launch_tiles<HD, QT, KT, false>(p, a.big_slots, a.big_splits, work + big_at, st)));
-    if (a.small) AR_TRY((launch_tiles<HD, QT, KT, true>(p, a.small_slots, a.small_splits, work, st)));
-    return AR_HIP_OK;
-}
-
 template <int HD, typename QT>
-int launch_kt(int dtype, const Plan& a, const PagedParams& p, char* work, size_t big_at, hipStream_t st) {
-    if (dtype == AR_DTYPE_F32) return launch_plan<HD, QT, float>(a, p, work, big_at, st);
-    if (dtype == AR_DTYPE_F16) return launch_plan<HD, QT, _Float16>(a, p, work, big_at, st);
-    return launch_plan<HD, QT, __hip_bfloat16>(a, p, work, big_at, st);
+int launch_kt(const ar_pages* pages, const Plan& a, const PagedParams& p, char* work, hipStream_t st) {
+    if (pages->dtype == AR_DTYPE_F32) return launch_plan<HD, QT, float>(pages, a, p, work, st);
+    if (pages->dtype == AR_DTYPE_F16) return launch_plan<HD, QT, _Float16>(pages, a, p, work, st);
+    return launch_plan<HD, QT, __hip_bfloat16>(pages, a, p, work, st);
 }
 
 int check_attention(const ar_pages* pages, const ar_chunks* chunks, int heads, const char* what) {
@@ -713,7 +1089,7 @@ extern "C" int ar_hip_attention_paged_work(ar_hip_ctx* ctx, const ar_pages* page
     AR_CHECK_ARG(ctx, "ctx is null");
     Plan a;
     AR_TRY(plan_of(ctx, pages, chunks, heads, &a));
-    *bytes = a.bytes;
+    *bytes = plan_bytes(pages, a);
     return AR_HIP_OK;
 }
 
@@ -730,7 +1106,8 @@ extern "C" int ar_hip_attention_paged(ar_hip_ctx* ctx, const ar_pages* pages, in
     if (chunks->rows == 0) return AR_HIP_OK;
     Plan a;
     AR_TRY(plan_of(ctx, pages, chunks, heads, &a));
-    AR_CHECK_ARG(work && work_bytes >= a.bytes, "%s: %zu bytes of work space given, %zu needed", what, work ? work_bytes : 0, a.bytes);
+    const size_t need = plan_bytes(pages, a);
+    AR_CHECK_ARG(work && work_bytes >= need, "%s: %zu bytes of work space given, %zu needed", what, work ? work_bytes : 0, need);
     const int hd = pages->head_dim;
     const size_t act = act_dtype == AR_DTYPE_F32 ? 4 : 2, bytes = (size_t)chunks->rows * heads * hd * act;
     if (ar_check_ptrs_enabled()) {
@@ -738,7 +1115,7 @@ extern "C" int ar_hip_attention_paged(ar_hip_ctx* ctx, const ar_pages* pages, in
         AR_TRY(page_check_chunk_ranges(chunks, what));
         AR_TRY(ar_check_range(q, bytes, what, "queries"));
         AR_TRY(ar_check_range(out, bytes, what, "output"));
-        AR_TRY(ar_check_range(work, a.bytes, what, "work space"));
+        AR_TRY(ar_check_range(work, need, what, "work space"));
     }
     const size_t layer_bytes = (size_t)pages->pages * pages->kv_heads * hd * pages->page_rows * page_elem_bytes(pages->dtype);
     PagedParams p{};
@@ -748,13 +1125,12 @@ extern "C" int ar_hip_attention_paged(ar_hip_ctx* ctx, const ar_pages* pages, in
     p.table = pages->table; p.seq = chunks->seq; p.start = chunks->start; p.at = chunks->at; p.heads = heads;
     p.kv_heads = pages->kv_heads; p.group = heads / pages->kv_heads; p.seqs = pages->seqs;
     p.max_pages = pages->max_pages; p.pages = pages->pages; p.shift = page_shift_of(pages); p.n = chunks->n;
-    p.rows = chunks->rows; p.small_rows = a.small_rows;
+    p.rows = chunks->rows; p.few_rows = a.few_rows;
     p.scale = (float)(1.4426950408889634 / std::sqrt((double)hd));
-    const size_t big_at = part_bytes(pages, a.small_slots, a.small_splits, 32);
     char* const w = (char*)work;
     if (hd == 128)
-        return act == 4 ? launch_kt<128, float>(pages->dtype, a, p, w, big_at, ctx->stream)
-                        : launch_kt<128, __hip_bfloat16>(pages->dtype, a, p, w, big_at, ctx->stream);
-    return act == 4 ? launch_kt<64, float>(pages->dtype, a, p, w, big_at, ctx->stream)
-                    : launch_kt<64, __hip_bfloat16>(pages->dtype, a, p, w, big_at, ctx->stream);
+        return act == 4 ? launch_kt<128, float>(pages, a, p, w, ctx->stream)
+                        : launch_kt<128, __hip_bfloat16>(pages, a, p, w, ctx->stream);
+    return act == 4 ? launch_kt<64, float>(pages, a, p, w, ctx->stream)
+                    : launch_kt<64, __hip_bfloat16>(pages, a, p, w, ctx->stream);
 }

@@ -456,7 +456,7 @@ int page_check(const ar_pages* p, bool table, const char* what) {
                  "%s: more than 4096 layers, 4096 KV heads or 2^28 pages", what);
     AR_CHECK_ARG(p->seqs >= 0 && p->seqs < 1 << 30 && p->max_pages >= 0, "%s: table of %d sequences, %d pages each", what,
                  p->seqs, p->max_pages);
-    AR_CHECK_ARG((long long)p->max_pages * p->page_rows <= 0x7fffffffLL, "%s: table rows of %d pages of %d rows pass 2^31",
+    AR_CHECK_ARG((long long)p->max_pages * p->page_rows <= 1LL << 30, "%s: table rows of %d pages of %d rows pass 2^30",
                  what, p->max_pages, p->page_rows);
     AR_CHECK_ARG(!table || (p->table && p->seqs > 0 && p->max_pages > 0), "%s: the pool has no table", what);
     return AR_HIP_OK;

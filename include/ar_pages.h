@@ -40,7 +40,7 @@ typedef struct ar_pages {
     int32_t page_rows;  /* a power of two, 16 .. 256 */
     int32_t head_dim;   /* 64 or 128 */
     int32_t seqs;       /* table rows; 0 with a null table for a pool alone (ar_hip_pages_copy) */
-    int32_t max_pages;  /* table columns; max_pages * page_rows < 2^31 */
+    int32_t max_pages;  /* table columns; max_pages * page_rows <= 2^30 */
 } ar_pages;
 
 /* The new rows of a call, by sequence: chunk i is the rows start[i] .. start[i+1]-1 of the call's row arrays, and

@@ -71,7 +71,7 @@ def _attend(p, c, layer=0, q=A, act=0, heads=4, out=A, work=A, bytes_=1 << 30):
 BAD_POOLS = [(dict(k=None), "no keys"), (dict(v=A + 4), "aligned"), (dict(dtype=3), "dtype"), (dict(head_dim=96), "head_dim"),
              (dict(page_rows=48), "power of two"), (dict(page_rows=8), "power of two"), (dict(page_rows=512), "power of two"),
              (dict(layers=0), "empty"), (dict(pages=0), "empty"), (dict(pages=-1), "empty"), (dict(kv_heads=0), "empty"),
-             (dict(pages=(1 << 28) + 1), "2^28"), (dict(seqs=-1), "table"), (dict(max_pages=1 << 28), "2^31")]
+             (dict(pages=(1 << 28) + 1), "2^28"), (dict(seqs=-1), "table"), (dict(max_pages=1 << 28), "2^30")]
 
 
 @pytest.mark.parametrize("over,word", BAD_POOLS)
