@@ -80,14 +80,15 @@ struct Elem<true> {
     static constexpr unsigned kExponent = 0x7C00;
 };
 
-// N planes of two values: v = plane 0 + plane 1 + ...  (an infinity or NaN is in plane 0 alone)
-template <bool F16, int N>
+// N planes of two values: v = plane 0 + plane 1 + ...  (SPECIAL: an infinity or NaN is in plane 0 alone)
+template <bool F16, int N, bool SPECIAL>
 __device__ __forceinline__ void split2(float x, float y, unsigned* out) {
     typedef Elem<F16> E;
     out[0] = E::pack(x, y);
     if constexpr (N > 1) {
-        x = fabsf(x) < INFINITY ? x - E::low(out[0]) : 0.f;
-        y = fabsf(y) < INFINITY ? y - E::high(out[0]) : 0.f;
+        const bool fx = !SPECIAL || fabsf(x) < INFINITY, fy = !SPECIAL || fabsf(y) < INFINITY;
+        x = fx ? x - E::low(out[0]) : 0.f;
+        y = fy ? y - E::high(out[0]) : 0.f;
         out[1] = E::pack(x, y);
     }
     if constexpr (N > 2) out[2] = E::pack(x - E::low(out[1]), y - E::high(out[1]));
@@ -99,9 +100,18 @@ __device__ __forceinline__ floatx4 mac4f(unsigned a, float b, floatx4 c) {
 }
 __device__ __forceinline__ floatx4 mac4(unsigned a, unsigned b, floatx4 c) { return mac4f(a, __uint_as_float(b), c); }
 
-// Power of two that brings a row whose largest value is `top` into fp16's range, its largest to [2^14, 2^15).
-__device__ __forceinline__ int fp16_shift(float top) {
-    return top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 100) : 0;
+// Power of two that brings a row whose largest finite value is `top` into fp16's range, its largest to [2^14, 2^15);
+// at most 2^100, also for a row of zeros.
+__device__ __forceinline__ int fp16_shift(float top) { return min(141 - (int)(__float_as_uint(top) >> 23), 100); }
+
+// maximum over the LANES (8 or 16) lanes that hold a row
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_mov<0xB1, 0xF>(v));   // quad_perm 1,0,3,2
+    v = fmaxf(v, dpp_mov<0x4E, 0xF>(v));   // quad_perm 2,3,0,1
+    v = fmaxf(v, dpp_mov<0x141, 0xF>(v));  // row_half_mirror
+    if (LANES == 16) v = fmaxf(v, dpp_mov<0x140, 0xF>(v));  // row_mirror
+    return v;
 }
 
 // A piece of values (of fp32 or 16-bit ones) with zeros for infinities and NaN, which a hidden key's weight of 0 would
@@ -138,13 +148,16 @@ template <>
 struct Kind<_Float16> { static constexpr int id = AR_DTYPE_F16; };
 
 constexpr int kThreads = 256, kWaves = 4;
+// The tile kernel's maximum of a row may lag behind by this power of two: weights up to 2^kSlack (fp16: 2^14).
+constexpr float kSlack = 8.f;
 
 // Planes and sizes of a (head size, activation, cache) combination.
 template <int HD, typename QT, typename KT>
 struct Shape {
-    static constexpr bool F16 = Kind<KT>::id == AR_DTYPE_F16, QF = Kind<QT>::id == AR_DTYPE_F32, KF = Kind<KT>::id == AR_DTYPE_F32;
+    static constexpr bool QF = Kind<QT>::id == AR_DTYPE_F32, KF = Kind<KT>::id == AR_DTYPE_F32;
+    static constexpr bool F16 = Kind<KT>::id != AR_DTYPE_BF16;
     static constexpr int NQ = !QF ? 1 : F16 ? 2 : 3;      // planes of queries and of weights
-    static constexpr int NK = !KF ? 1 : QF ? 3 : 2;       // planes of keys and values
+    static constexpr int NK = KF ? 2 : 1;                 // planes of keys and values
     static constexpr int DEPTH = NQ > NK ? NQ : NK;       // plane pairs (i, j) with i + j < DEPTH are multiplied
     static constexpr int CPR = HD / 8;                    // 8-value pieces of a row
     // the tile kernel: 128 packed rows a block, 32 a wavefront, key tiles of BK shared by the block
@@ -153,40 +166,27 @@ struct Shape {
     static constexpr int UNITS = BK * CPR / kThreads;     // pieces of a tile per thread
     static constexpr int PLANE = BK * HD * 2;             // bytes of a plane of a tile
     static constexpr int TILE = NK * PLANE;
-    static constexpr float BIAS = F16 ? 14.f : 0.f;  // weights scaled by 2^14 in fp16: their small ones keep bits
+    static constexpr float BIAS = F16 ? 6.f : 0.f;  // weights scaled by 2^6 in fp16, and kSlack more: their small ones keep bits
 };
 
 // ---- what a block works on --------------------------------------------------------------------------------------
-// Tasks are the tiles of ROWS packed rows of every chunk, in the key splits of `per` units of kUnit keys.  Where there
-// are enough tiles to fill the GPU a task is a tile (p.target 0): the block's slot is searched among the chunks, 64 at a
-// time.  Otherwise every block adds up all chunks' units, so that `per` makes about p.target tasks of equal length
-// whatever the lengths of the sequences are, and finds its task in their order.
-constexpr int kUnit = 128;
+// Tasks are the tiles of ROWS packed rows of every chunk.  Where there are enough of them to fill the GPU, a tile is a task
+// (p.target 0): the block's slot is searched among the chunks, 64 at a time.  Otherwise every block adds up what all
+// chunks' tiles see, so that splits of `per` units of kUnit<ROWS> keys make about p.target tasks of equal length whatever
+// the lengths of the sequences are, and finds its task in their order.  In a chunk of several tiles, tile j's tasks begin
+// at floor(S(j) / L) + 2 j, with L keys in a split and S(j) the keys that the tiles before j see, from above and in closed
+// form: at least as many as its splits, and found without a sum over tiles; those past its splits are empty.
+template <int ROWS>
+constexpr int kUnit = ROWS == 16 ? 128 : 64;  // a round of the few-row kernel's wavefronts; the tile kernel's largest key tile
 
 struct Task {
     int seq, first, count;  // chunk
-    long long at;           // cache row of its first token
+    int at;                 // cache row of its first token
     int r0, rows;           // packed rows: first, and how many there are
     int units;              // key units its chunk's last row sees
     int per, splits, split; // units of a split, splits, and which
     int base;               // the tile's first task
 };
-
-// Chunk i's rows, sequence and place; the number of its tiles (0: not this kernel's).
-template <int ROWS>
-__device__ __forceinline__ int chunk_tiles(const PagedParams& p, int i, Task* t) {
-    chunk_rows(p.start, i, p.rows, &t->first, &t->count);
-    const long long packed = (long long)t->count * p.group;
-    t->seq = p.seq ? p.seq[i] : i;
-    t->at = p.at[i];
-    const long long cap = (long long)p.max_pages << p.shift;
-    long long end = t->at + t->count;
-    if (end > cap) end = cap;
-    if (t->at < 0 || t->seq < 0 || t->seq >= p.seqs) end = 0;
-    t->units = (int)((end + kUnit - 1) / kUnit);
-    if (t->count == 0 || (ROWS == 16 ? packed > p.few_rows : packed <= p.few_rows)) return 0;
-    return (int)((packed + ROWS - 1) / ROWS);
-}
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // The table is read with scalar loads: nothing writes it while these kernels run.
@@ -195,27 +195,67 @@ __device__ __forceinline__ TableRow table_row(const PagedParams& p, int seq) {
     return (TableRow)(uintptr_t)(p.table + (size_t)(seq < 0 ? 0 : seq) * p.max_pages);
 }
 
-__device__ __forceinline__ long long wave_sum(long long v) {
+// Chunk i's rows, sequence and place; the number of its tiles (0: not this kernel's, or i past the last chunk).
+template <int ROWS>
+__device__ __forceinline__ int chunk_tiles(const PagedParams& p, int i, Task* t) {
+    const int j = min(i, p.n - 1);
+    // (all loads at once)
+    const int a = p.start ? p.start[j] : j, b = p.start ? p.start[j + 1] : j + 1;
+    const int at = p.at[j], seq = p.seq ? p.seq[j] : j;
+    t->first = a;
+    t->count = i < p.n && a >= 0 && b > a && b <= p.rows ? b - a : 0;
+    t->seq = seq;
+    t->at = at;
+    const int cap = p.max_pages << p.shift;  // (at most 2^30)
+    const int end = at < 0 || seq < 0 || seq >= p.seqs ? 0 : at >= cap ? cap : min(at + t->count, cap);
+    t->units = (end + kUnit<ROWS> - 1) / kUnit<ROWS>;
+    const int packed = t->count * p.group;  // (at most 2^30)
+    if (t->count == 0 || (ROWS == 16 ? packed > p.few_rows : packed <= p.few_rows)) return 0;
+    return (packed + ROWS - 1) / ROWS;
+}
+
+// Keys that tile j of the chunk's n sees; S(j) above; first task of tile j.
+template <int ROWS>
+__device__ __forceinline__ int tile_end(const PagedParams& p, const Task& c, int j) {
+    const int cap = p.max_pages << p.shift, packed = c.count * p.group;
+    return c.units == 0 ? 0 : c.at >= cap ? cap : min(c.at + (min((j + 1) * ROWS, packed) - 1) / p.group + 1, cap);
+}
+template <int ROWS>
+__device__ __forceinline__ double keys_before(const PagedParams& p, const Task& c, int j) {
+    const double at = min(c.at, p.max_pages << p.shift) + 1;
+    return c.units == 0 ? 0. : j * at + 0.5 * ROWS * j * (j + 1.) / p.group;
+}
+template <int ROWS>
+__device__ __forceinline__ int first_task(const PagedParams& p, const Task& c, int j, double inv) {
+    return (int)(keys_before<ROWS>(p, c, j) * inv) + 2 * j;
+}
+
+// Sum over the wavefront, and of the lanes up to and with this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_up(v, d);
+        if (lane >= d) v += x;
+    }
     return v;
 }
 
-// Task `index` (MERGE: tile `index` of those with several splits or one) -> *t, by one wavefront; every wavefront of a
-// block computes it for itself.
+// Task `index` (MERGE: tile `index` and its first task) -> *t, by one wavefront; every wavefront of a block computes it
+// for itself.
 template <int ROWS, bool MERGE>
 __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task* t) {
     const int lane = threadIdx.x & 63;
-    int tile;
+    int tile = 0;
     if (p.target == 0) {
-        const int chunk = !p.start ? index / ((p.group + ROWS - 1) / ROWS) : chunk_search(p.n, 64, [&](int i, int k, int len) {
+        const int per_chunk = (p.group + ROWS - 1) / ROWS;
+        const int chunk = !p.start ? index / per_chunk : chunk_search(p.n, 64, [&](int i, int k, int len) {
             const bool below = (long long)lane * k < len && chunk_slot(p.start[i + lane * k], i + lane * k, p.group, ROWS) <= index;
             const unsigned long long m = __ballot(below);
             return m == ~0ull ? 64 : __builtin_ctzll(~m);
         });
-        if (chunk >= p.n) return false;
         const int tiles = chunk_tiles<ROWS>(p, chunk, t);
-        const long long at = !p.start ? index % ((p.group + ROWS - 1) / ROWS) : index - chunk_slot(t->first, chunk, p.group, ROWS);
+        const long long at = !p.start ? index % per_chunk : index - chunk_slot(t->first, chunk, p.group, ROWS);
         if (at < 0 || at >= tiles) return false;
         tile = (int)at;
         t->per = t->units > 0 ? t->units : 1;
@@ -223,65 +263,84 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         t->split = 0;
         t->base = index;
     } else {
-        long long units = 0;
-        for (int i = lane; i < p.n; i += 64) {
-            Task c;
-            units += (long long)chunk_tiles<ROWS>(p, i, &c) * c.units;
+        // (of up to 64 chunks each lane keeps its own)
+        Task c;
+        int n = chunk_tiles<ROWS>(p, lane, &c);
+        double keys = keys_before<ROWS>(p, c, n);
+        for (int i = lane + 64; i < p.n; i += 64) {
+            Task d;
+            const int k = chunk_tiles<ROWS>(p, i, &d);
+            keys += keys_before<ROWS>(p, d, k);
         }
-        units = wave_sum(units);
-        const int per = max(1, (int)((units + p.target - 1) / p.target));
-        long long tasks = 0, tiles = 0;  // before this round's chunks
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) keys += __shfl_xor(keys, d);
+        const int per = (int)fmax(1., fmin(ceil(keys / ((double)p.target * kUnit<ROWS>)), 1 << 24));
+        const double inv = 1. / ((double)per * kUnit<ROWS>);
+        int tasks = 0, tiles = 0;  // before this round's chunks
         bool found = false;
         for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
-            Task c;
-            int n = 0, s = 1;
-            if (i0 + lane < p.n) {
-                n = chunk_tiles<ROWS>(p, i0 + lane, &c);
-                s = max(1, (c.units + per - 1) / per);
-            }
-            long long a = (long long)n * s, b = n;  // tasks and tiles up to and with this lane's chunk
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const long long x = __shfl_up(a, d), y = __shfl_up(b, d);
-                if (lane >= d) {
-                    a += x;
-                    b += y;
-                }
-            }
+            if (i0) n = chunk_tiles<ROWS>(p, i0 + lane, &c);
+            const int mine = n == 0 ? 0 : n == 1 ? max(1, (c.units + per - 1) / per) : first_task<ROWS>(p, c, n, inv);
+            const int a = wave_scan(mine), b = wave_scan(n);  // with this lane's chunk
             const unsigned long long m = __ballot((MERGE ? tiles + b : tasks + a) > index);
             if (m) {
                 const int l = __builtin_ctzll(m);
-                const int chunk = i0 + l;
-                chunk_tiles<ROWS>(p, chunk, t);
-                n = __shfl(n, l);
-                t->splits = __shfl(s, l);
-                const long long a0 = tasks + __shfl(a, l) - (long long)n * t->splits, b0 = tiles + __shfl(b, l) - n;
-                const int at = (int)(index - (MERGE ? b0 : a0));
-                // (a tile's splits one after another)
-                tile = MERGE ? at : at / t->splits;
-                t->split = MERGE ? 0 : at - tile * t->splits;
-                t->base = (int)(a0 + (long long)tile * t->splits);
+                t->first = __shfl(c.first, l);
+                t->count = __shfl(c.count, l);
+                t->seq = __shfl(c.seq, l);
+                t->at = __shfl(c.at, l);
+                t->units = __shfl(c.units, l);
+                const int all = __shfl(n, l), a0 = tasks + __shfl(a, l) - __shfl(mine, l), b0 = tiles + __shfl(b, l) - all;
+                const int q = index - (MERGE ? b0 : a0);
+                if (MERGE || all == 1) {
+                    tile = MERGE ? q : 0;
+                } else {
+                    int hi = all - 1;  // the last tile whose tasks begin at q or before
+                    while (tile < hi) {
+                        const int mid = tile + (hi - tile + 1) / 2;
+                        if (first_task<ROWS>(p, *t, mid, inv) <= q) tile = mid;
+                        else hi = mid - 1;
+                    }
+                }
+                const int begin = all == 1 ? 0 : first_task<ROWS>(p, *t, tile, inv);
+                const int units = (tile_end<ROWS>(p, *t, tile) + kUnit<ROWS> - 1) / kUnit<ROWS>;
+                t->splits = max(1, (units + per - 1) / per);
+                t->split = MERGE ? 0 : q - begin;
+                t->base = a0 + begin;
                 found = true;
             }
             tasks += __shfl(a, 63);
             tiles += __shfl(b, 63);
         }
-        if (!found) return false;
+        if (!found || t->split >= t->splits) return false;
         t->per = per;
     }
-    // (the same in every lane, and so in scalar registers)
-    t->seq = uniform(t->seq);
-    t->first = uniform(t->first);
-    t->count = uniform(t->count);
-    t->at = uniform((int)t->at);
-    t->units = uniform(t->units);
-    t->per = uniform(t->per);
-    t->splits = uniform(t->splits);
-    t->split = uniform(t->split);
-    t->base = uniform(t->base);
-    t->r0 = uniform(tile * ROWS);
+    t->r0 = tile * ROWS;
     t->rows = min(t->count * p.group - t->r0, ROWS);
     return true;
+}
+
+// Says that a found task is the same in every lane: its fields go into scalar registers, and so does what follows from
+// them (behind the branch on whether there is one: values that meet behind it count as different).
+__device__ __forceinline__ Task settled(Task t) {
+    t.seq = uniform(t.seq);
+    t.first = uniform(t.first);
+    t.count = uniform(t.count);
+    t.at = uniform(t.at);
+    t.r0 = uniform(t.r0);
+    t.rows = uniform(t.rows);
+    t.units = uniform(t.units);
+    t.per = uniform(t.per);
+    t.splits = uniform(t.splits);
+    t.split = uniform(t.split);
+    t.base = uniform(t.base);
+    return t;
+}
+
+// The last key that packed row r of the task's chunk sees, -1: none.
+__device__ __forceinline__ int last_key(const PagedParams& p, const Task& t, int r) {
+    const int cap = p.max_pages << p.shift;
+    return t.units == 0 ? -1 : t.at >= cap ? cap - 1 : min(t.at + r / p.group, cap - 1);
 }
 
 template <typename QT>
@@ -316,32 +375,183 @@ __device__ __forceinline__ void store4(__hip_bfloat16* p, float a, float b, floa
     *reinterpret_cast<uint2*>(p) = make_uint2(Elem<false>::pack(a, b), Elem<false>::pack(c, d));
 }
 
+// A barrier over LDS only: loads from memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <int HD, typename QT, typename KT>
 __global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p) {
     typedef Shape<HD, QT, KT> C;
     typedef Elem<C::F16> E;
     constexpr int NQ = C::NQ, NK = C::NK, BK = C::BK, KT32 = BK / 32, NJ = HD / 32, KS = HD / 16;
-    __shared__ __attribute__((aligned(16))) char lds[2 * C::TILE];
-    __shared__ int s_bad;
+    __shared__ __attribute__((aligned(16))) char lds[4 * C::TILE];  // keys and values of a tile and of the next
+    __shared__ __attribute__((aligned(16))) int s_exp[2][2][BK];    // fp32 caches: powers of two that they carry
+    __shared__ int s_bad[2];
 
     const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // KV head fastest (8 of them: one to an XCD, whose L2 then holds that head's rows), later rows, with more keys, first
     const int kvh = blockIdx.x % p.kv_heads;
-    Task t;
-    if (!find_task<C::ROWS, false>(p, p.tasks - 1 - (int)(blockIdx.x / p.kv_heads), &t)) return;
+    Task found;
+    if (!find_task<C::ROWS, false>(p, p.tasks - 1 - (int)(blockIdx.x / p.kv_heads), &found)) return;
+    const Task t = settled(found);
 
     const int row = t.r0 + 32 * wave + lq, packed = t.r0 + t.rows;  // row: packed, in the chunk
     const bool mine = row < packed;
     const int tok = mine ? row / p.group : 0, head = kvh * p.group + (mine ? row - tok * p.group : 0);
     const size_t qrow = ((size_t)(t.first + tok) * p.heads + head) * HD;
-    const long long cap = (long long)p.max_pages << p.shift;
-    auto last_key = [&](int r) { return t.units == 0 ? -1 : (int)(t.at + r / p.group < cap ? t.at + r / p.group : cap - 1); };
     // the last key a row sees; the wavefront's first and last rows', the block's
     const int w0 = t.r0 + 32 * wave;
-    const int lim = mine ? last_key(row) : -1, lim0 = w0 < packed ? last_key(w0) : -1;
-    const int lim1 = w0 < packed ? last_key(min(w0 + 31, packed - 1)) : -1;
-    const int blim0 = last_key(t.r0), kend = last_key(packed - 1) + 1;
+    const int lim = mine ? last_key(p, t, row) : -1, lim0 = uniform(w0 < packed ? last_key(p, t, w0) : -1);
+    const int lim1 = uniform(w0 < packed ? last_key(p, t, min(w0 + 31, packed - 1)) : -1);
+    const int blim0 = uniform(last_key(p, t, t.r0)), kend = uniform(last_key(p, t, packed - 1)) + 1;
+
+    floatx16 o[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[j][r] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    int ve = 100;  // (fp32 caches) the outputs are times 2^ve
+
+    const int t0 = t.split * t.per * (kUnit<128> / BK), t1 = min(t0 + t.per * (kUnit<128> / BK), (kend + BK - 1) / BK);
+    const TableRow table = table_row(p, t.seq);
+    const int kmax = max(kend - 1, 0);
+    const int pmask = (1 << p.shift) - 1;
+
+    // swizzles of 16-byte pieces in a row: K, 16 rows of one column over all banks; V, 4 rows of 4 columns
+    const int kx = HD == 128 ? lq & 15 : (lq >> 1) & 7;
+    const unsigned kaddr = lq * (HD * 2) + ((h ^ kx) * 16);
+    const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2);
+    auto value_swizzle = [](int key) { return HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; };
+    const unsigned vaddr = vrow * (HD * 2) + (((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ value_swizzle(vrow)) * 16) + (i16 & 1) * 8;
+
+    // A wavefront's 64 pieces of a load lie in 64 / CPR rows of one page (its first row is a multiple of that, and pages
+    // are longer), so that all but a fixed offset of each lane's address is the same for the wavefront.
+    constexpr int ROW = HD * (int)sizeof(KT);
+    typedef u32x4 Staged[C::UNITS * (C::KF ? 2 : 1)];
+    Staged sk, sv;  // the next tile's keys and values, on their way
+    const unsigned lane_at = (lane / C::CPR) * ROW + (lane % C::CPR) * (8 * (int)sizeof(KT));
+    int pg0 = -1, pg1 = -1, pg2 = -1, pg3 = -1;
+    auto page_at = [&](int k0, int i) __attribute__((always_inline)) {
+        const int key = k0 + (i << p.shift), n = table[min(key, kmax) >> p.shift];
+        return (i << p.shift) < BK && key < kend && n >= 0 && n < p.pages ? n : -1;
+    };
+    auto load_pages = [&](int tile) __attribute__((always_inline)) {
+        const int k0 = tile * BK;
+        pg0 = page_at(k0, 0);
+        pg1 = page_at(k0, 1);
+        if constexpr (BK > 32) {
+            pg2 = page_at(k0, 2);
+            pg3 = page_at(k0, 3);
+        }
+    };
+    // (a row on no page: some row of the pool in its place; keys are hidden by their scores, values zeroed below)
+    auto stage_load = [&](Staged& st, int tile, const char* pool, int a0, int a1, int a2, int a3) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < C::UNITS; u++) {
+            const int row0 = (u * kThreads + wave * 64) / C::CPR, i = row0 >> p.shift;
+            int page = i >= 1 ? a1 : a0;
+            page = i >= 2 ? a2 : page;
+            page = i >= 3 ? a3 : page;
+            page = page < 0 ? 0 : page;
+            const char* src = pool + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((tile * BK + row0) & pmask)) * ROW;
+            if constexpr (C::KF) {
+                st[2 * u] = *reinterpret_cast<const u32x4*>(src + lane_at);
+                st[2 * u + 1] = *reinterpret_cast<const u32x4*>(src + lane_at + 16);
+            } else {
+                st[u] = *reinterpret_cast<const u32x4*>(src + lane_at);
+            }
+        }
+    };
+    auto stage_store = [&](const Staged& st, int odd, int values) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < C::UNITS; u++) {
+            const int piece = u * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
+            const int x = values ? value_swizzle(key) : HD == 128 ? key & 15 : (key >> 1) & 7;
+            char* dst = lds + (2 * odd + values) * C::TILE + key * (HD * 2) + ((col ^ x) * 16);
+            if constexpr (C::KF) {
+                float v[8], top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[i] = __uint_as_float(st[2 * u + i / 4][i % 4]);
+                    top = fmaxf(top, fabsf(v[i]));
+                }
+                float sum = 0.f;  // (NaN where there is one)
+#pragma unroll
+                for (int i = 0; i < 8; i++) sum = fmaf(v[i], 0.f, sum);
+                top = row_max<C::CPR>(top);
+                const bool special = __ballot(!(top < INFINITY) || sum != 0.f);
+                if (__builtin_expect(special, 0)) {  // the largest finite value of the row
+                    top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
+                    top = row_max<C::CPR>(top);
+                }
+                const int e = fp16_shift(top);
+                const float scale = __uint_as_float((unsigned)(e + 127) << 23);
+                unsigned pl[4][NK];
+#pragma unroll
+                for (int i = 0; i < 4; i++) split2<true, NK, false>(v[2 * i] * scale, v[2 * i + 1] * scale, pl[i]);
+                if (__builtin_expect(special, 0)) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) split2<true, NK, true>(v[2 * i] * scale, v[2 * i + 1] * scale, pl[i]);
+                }
+#pragma unroll
+                for (int n = 0; n < NK; n++)
+                    *reinterpret_cast<u32x4*>(dst + n * C::PLANE) = quad(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
+                if (col == 0) s_exp[odd][values][key] = e;
+            } else {
+                *reinterpret_cast<u32x4*>(dst) = st[u];
+            }
+        }
+    };
+    // Zeros this thread's pieces of values that are not there, infinities and NaN, in LDS; whether there were any of
+    // these.  (Few tiles need it: a loop, and in LDS, for the sake of the others' registers.)
+    auto clean = [&](int odd, int k0, unsigned long long miss) __attribute__((always_inline)) {
+        unsigned any = 0;
+#pragma unroll 1
+        for (int u = 0; u < C::UNITS * NK; u++) {
+            const int piece = u / NK * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
+            u32x4* const at = reinterpret_cast<u32x4*>(lds + (2 * odd + 1) * C::TILE + u % NK * C::PLANE + key * (HD * 2) +
+                                                    ((col ^ value_swizzle(key)) * 16));
+            const bool out = k0 + key >= kend || (miss >> key & 1);
+            any |= leave_out<C::F16>(at, out);
+            if (C::KF && out) s_exp[odd][1][key] = 100;
+        }
+        return any != 0;
+    };
+
+    // keys of a tile that lie on no page (or behind the last key), by its pages
+    auto missing = [&]() __attribute__((always_inline)) {
+        const unsigned long long page_keys = p.shift >= 6 ? ~0ull : (1ull << (1 << p.shift)) - 1;
+        unsigned long long miss = 0;
+        if (pg0 < 0) miss |= page_keys;
+        if (pg1 < 0 && (1 << p.shift) < BK) miss |= page_keys << ((1 << p.shift) & 63);
+        if (pg2 < 0 && (2 << p.shift) < BK) miss |= page_keys << ((2 << p.shift) & 63);
+        if (pg3 < 0 && (3 << p.shift) < BK) miss |= page_keys << ((3 << p.shift) & 63);
+        return miss;
+    };
+    // The staged tile into LDS; where some row of the block does not see all of it, its values are cleaned.
+    auto stage_tile = [&](int tile, unsigned long long miss) __attribute__((always_inline)) {
+        const int odd = tile & 1;
+        stage_store(sk, odd, 0);
+        stage_store(sv, odd, 1);
+        if (tile < t1 && (miss != 0 || tile * BK + BK - 1 > blim0) && clean(odd, tile * BK, miss)) s_bad[odd] = tile;
+    };
+
+    if (tid < 2) s_bad[tid] = -1;
+    __syncthreads();
+    load_pages(t0);
+    unsigned long long miss = missing();
+    if (t0 < t1) {
+        stage_load(sk, t0, p.kp, pg0, pg1, pg2, pg3);
+        stage_load(sv, t0, p.vp, pg0, pg1, pg2, pg3);
+    }
 
     // queries: planes in registers, rows of an fp16 cache's scaled into its range
     u32x4 qf[NQ][KS];
@@ -361,7 +571,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p)
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[s][i]));
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[s][i]) < INFINITY ? fabsf(v[s][i]) : 0.f);
             top = max_xor32(top);
             const int e = fp16_shift(top);
             c = ldexpf(c, -e);
@@ -374,240 +584,227 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p)
         for (int s = 0; s < KS; s++) {
             unsigned u[4][NQ];
 #pragma unroll
-            for (int i = 0; i < 4; i++) split2<C::F16, NQ>(v[s][2 * i], v[s][2 * i + 1], u[i]);
+            for (int i = 0; i < 4; i++) split2<C::F16, NQ, true>(v[s][2 * i], v[s][2 * i + 1], u[i]);
 #pragma unroll
             for (int n = 0; n < NQ; n++) qf[n][s] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
         }
     }
 
-    floatx16 o[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; j++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) o[j][r] = 0.f;
-    float m = -INFINITY, l = 0.f;
-
-    const int t0 = t.split * t.per * (kUnit / BK), t1 = min(t0 + t.per * (kUnit / BK), (kend + BK - 1) / BK);
-    const TableRow table = table_row(p, t.seq);
-    const int kmax = max(kend - 1, 0);
-    const int pmask = (1 << p.shift) - 1;
-
-    char* const kbuf = lds;
-    char* const vbuf = lds + C::TILE;
-    // swizzles of 16-byte pieces in a row: K, 16 rows of one column over all banks; V, 4 rows of 4 columns
-    const int kx = HD == 128 ? lq & 15 : (lq >> 1) & 7;
-    const unsigned kaddr = lq * (HD * 2) + ((h ^ kx) * 16);
-    const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2);
-    auto value_swizzle = [](int key) { return HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; };
-    const unsigned vaddr = vrow * (HD * 2) + (((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ value_swizzle(vrow)) * 16) + (i16 & 1) * 8;
-
-    // A wavefront's 64 pieces of a load lie in 64 / CPR rows of one page (its first row is a multiple of that, and pages
-    // are longer), so that all but a fixed offset of each lane's address is the same for the wavefront.
-    constexpr int ROW = HD * (int)sizeof(KT);
-    u32x4 st[C::UNITS * (C::KF ? 2 : 1)];
-    const unsigned lane_at = (lane / C::CPR) * ROW + (lane % C::CPR) * (8 * (int)sizeof(KT));
-    int pg0 = -1, pg1 = -1, pg2 = -1, pg3 = -1;
-    auto page_at = [&](int k0, int i) __attribute__((always_inline)) {
-        const int key = k0 + (i << p.shift), n = table[min(key, kmax) >> p.shift];
-        return (i << p.shift) < BK && key < kend && n >= 0 && n < p.pages ? n : -1;
-    };
-    auto load_pages = [&](int tile) __attribute__((always_inline)) {
-        const int k0 = tile * BK;
-        pg0 = page_at(k0, 0);
-        pg1 = page_at(k0, 1);
-        if constexpr (BK > 32) {
-            pg2 = page_at(k0, 2);
-            pg3 = page_at(k0, 3);
-        }
-    };
-    // (a row on no page: some row of the pool in its place; keys are hidden by their scores, values zeroed below)
-    auto stage_load = [&](int tile, const char* pool, int a0, int a1, int a2, int a3) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < C::UNITS; u++) {
-            const int row0 = (u * kThreads + wave * 64) / C::CPR, i = row0 >> p.shift;
-            int page = i >= 1 ? a1 : a0;
-            page = i >= 2 ? a2 : page;
-            page = i >= 3 ? a3 : page;
-            page = page < 0 ? 0 : page;
-            const char* src = pool + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((tile * BK + row0) & pmask)) * ROW;
-            if constexpr (C::KF) {
-                st[2 * u] = *reinterpret_cast<const u32x4*>(src + lane_at);
-                st[2 * u + 1] = *reinterpret_cast<const u32x4*>(src + lane_at + 16);
-            } else {
-                st[u] = *reinterpret_cast<const u32x4*>(src + lane_at);
-            }
-        }
-    };
-    auto stage_store = [&](char* buf, bool values) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < C::UNITS; u++) {
-            const int piece = u * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
-            const int x = values ? value_swizzle(key) : HD == 128 ? key & 15 : (key >> 1) & 7;
-            char* dst = buf + key * (HD * 2) + ((col ^ x) * 16);
-            if constexpr (C::KF) {
-                const u32x4 a = st[2 * u], d = st[2 * u + 1];
-                const unsigned w[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
-                unsigned pl[4][NK];
-#pragma unroll
-                for (int i = 0; i < 4; i++) split2<false, NK>(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), pl[i]);
-#pragma unroll
-                for (int n = 0; n < NK; n++)
-                    *reinterpret_cast<u32x4*>(dst + n * C::PLANE) = quad(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
-            } else {
-                *reinterpret_cast<u32x4*>(dst) = st[u];
-            }
-        }
-    };
-    // Zeros this thread's pieces of values that are not there, infinities and NaN, in LDS; whether there were any of
-    // these.  (Few tiles need it: a loop, and in LDS, for the sake of the others' registers.)
-    auto clean = [&](int k0, unsigned long long miss) __attribute__((always_inline)) {
-        unsigned any = 0;
-#pragma unroll 1
-        for (int u = 0; u < C::UNITS * NK; u++) {
-            const int piece = u / NK * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
-            u32x4* const at = reinterpret_cast<u32x4*>(vbuf + u % NK * C::PLANE + key * (HD * 2) + ((col ^ value_swizzle(key)) * 16));
-            any |= leave_out<C::F16>(at, k0 + key >= kend || (miss >> key & 1));
-        }
-        return any != 0;
-    };
-
-    if (tid == 0) s_bad = -1;
+    unsigned long long miss_next = 0;
     if (t0 < t1) {
-        load_pages(t0);
-        stage_load(t0, p.kp, pg0, pg1, pg2, pg3);
+        load_pages(t0 + 1);
+        stage_tile(t0, miss);
+        miss_next = missing();
+        stage_load(sk, t0 + 1, p.kp, pg0, pg1, pg2, pg3);
+        stage_load(sv, t0 + 1, p.vp, pg0, pg1, pg2, pg3);
+        load_pages(t0 + 2);
     }
-    for (int tile = t0; tile < t1; tile++) {
-        const int k0 = tile * BK;
-        unsigned long long miss = 0;  // keys of the tile that lie on no page
-        const unsigned long long page_keys = p.shift >= 6 ? ~0ull : (1ull << (1 << p.shift)) - 1;
-        if (pg0 < 0) miss |= page_keys;
-        if (pg1 < 0 && (1 << p.shift) < BK) miss |= page_keys << ((1 << p.shift) & 63);
-        if (pg2 < 0 && (2 << p.shift) < BK) miss |= page_keys << ((2 << p.shift) & 63);
-        if (pg3 < 0 && (3 << p.shift) < BK) miss |= page_keys << ((3 << p.shift) & 63);
-        const bool masked = miss != 0 || k0 + BK - 1 > blim0;  // some row of the block does not see all of it
-        stage_store(kbuf, false);
-        stage_load(tile, p.vp, pg0, pg1, pg2, pg3);
-        load_pages(tile + 1);  // (past the split's end: not used)
-        __syncthreads();
 
-        const bool work = k0 <= lim1;
+    // One barrier a tile: behind it the tile is in LDS, and the one before it is done with; the next one goes from the
+    // registers into its place, and the loads of the one after that are issued, with a whole tile's time to arrive
+    // (past the split's end: rows that are not used).
+    for (int tile = t0; tile < t1; tile++) {
+        const int k0 = tile * BK, odd = tile & 1;
+        lds_barrier();
+        const bool bad = s_bad[odd] == tile;
+        stage_tile(tile + 1, miss_next);
+        stage_load(sk, tile + 2, p.kp, pg0, pg1, pg2, pg3);
+        stage_load(sv, tile + 2, p.vp, pg0, pg1, pg2, pg3);
+        const unsigned long long miss_here = miss;
+        miss = miss_next;
+        miss_next = missing();
+        load_pages(tile + 3);
+
+        const char* const kbuf = lds + 2 * odd * C::TILE;
+        const char* const vbuf = kbuf + C::TILE;
         floatx16 s[KT32];
-        if (work) {
+        auto scores = [&](int kt) __attribute__((always_inline)) {
 #pragma unroll
-            for (int kt = 0; kt < KT32; kt++) {
+            for (int r = 0; r < 16; r++) s[kt][r] = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[kt][r] = 0.f;
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
+                for (int j = 0; j < NK; j++) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + j * C::PLANE + kt * 32 * HD * 2 + (kaddr ^ (ks * 32)));
+#pragma unroll
+                    for (int i = 0; i < NQ; i++)
+                        if (i + j < C::DEPTH) s[kt] = E::mac(kf, qf[i][ks], s[kt]);
+                }
+        };
+        auto largest = [&](int kt) __attribute__((always_inline)) {
+            float mx = s[kt][0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
+            return mx;
+        };
+        // scores to weights; their sum, of this lane's half of the keys
+        auto weights = [&](int kt, float mu) __attribute__((always_inline)) {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], c, -mu));
+                sum[r & 3] += s[kt][r];
+            }
+            return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        };
+        auto products = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k2 = 0; k2 < 2; k2++) {
+                if (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // one step's planes at a time: registers
+                unsigned u[4][NQ];
+#pragma unroll
+                for (int i = 0; i < 4; i++) split2<C::F16, NQ, false>(s[kt][8 * k2 + 2 * i], s[kt][8 * k2 + 2 * i + 1], u[i]);
+                u32x4 pf[NQ];
+#pragma unroll
+                for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
+#pragma unroll
+                for (int jt = 0; jt < NJ; jt++)
 #pragma unroll
                     for (int j = 0; j < NK; j++) {
-                        const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + j * C::PLANE + kt * 32 * HD * 2 + (kaddr ^ (ks * 32)));
+                        const char* a = vbuf + j * C::PLANE + (vaddr ^ (jt * 64)) + (32 * kt + 16 * k2) * (HD * 2);
+                        typedef __attribute__((address_space(3))) shortx4 lds4;
+                        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a));
+                        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(a + 8 * HD * 2)));
+                        const u32x4 vf = quad(x.x, x.y, y.x, y.y);
 #pragma unroll
                         for (int i = 0; i < NQ; i++)
-                            if (i + j < C::DEPTH) s[kt] = E::mac(kf, qf[i][ks], s[kt]);
+                            if (i + j < C::DEPTH) o[jt] = E::mac(vf, pf[i], o[jt]);
                     }
+            }
+        };
+
+        if (k0 > lim1) continue;
+        // Tiles that every row sees in full, while no row's scores pass its maximum by much (most of them): the weights of
+        // a half are computed under the matrix instructions of the other half.
+        if constexpr (!C::KF) {
+            if (miss_here == 0 && k0 + BK - 1 <= lim0 && !bad) {
+                const float mu = m - C::BIAS;
+                if (NQ > 1) __builtin_amdgcn_s_setprio(1);  // (several planes: matrix instructions first)
+                scores(0);
+                if constexpr (KT32 > 1) scores(1);
+                if (NQ > 1) __builtin_amdgcn_s_setprio(0);
+                float mx = largest(0);
+                float sum = weights(0, mu);
+                if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
+                if (!__ballot(!(mx * c <= m + kSlack))) {
+                    if (NQ > 1) __builtin_amdgcn_s_setprio(1);
+                    products(0);
+                    if (NQ > 1) __builtin_amdgcn_s_setprio(0);
+                    if constexpr (KT32 > 1) {
+                        sum += weights(1, mu);
+                        products(1);
+                    }
+                    l += sum;
+                    continue;
                 }
             }
-            if (k0 + BK - 1 > lim0) {  // (the lane's keys are 32 kt + 8 (r / 4) + r % 4, and 4 h)
-                const int last = lim - k0 - 4 * h;
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT32; kt++) scores(kt);
+        if constexpr (C::KF) {
+#pragma unroll
+            for (int kt = 0; kt < KT32; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[kt][r] = ldexpf(s[kt][r], -s_exp[odd][0][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
+        }
+        if (k0 + BK - 1 > lim0) {  // (the lane's keys are 32 kt + 8 (r / 4) + r % 4, and 4 h)
+            asm volatile("");      // (a branch: few tiles have hidden keys)
+            const int last = lim - k0 - 4 * h;
+#pragma unroll
+            for (int kt = 0; kt < KT32; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (32 * kt + 8 * (r >> 2) + (r & 3) > last) s[kt][r] = -INFINITY;
+        }
+        if (miss_here != 0) {
+            asm volatile("");
+#pragma unroll
+            for (int kt = 0; kt < KT32; kt++) {
+                const unsigned gone = (unsigned)(miss_here >> (32 * kt)) >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (gone >> (8 * (r >> 2) + (r & 3)) & 1) s[kt][r] = -INFINITY;
+            }
+        }
+        float mx = largest(0);
+        if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
+        mx = max_xor32(mx) * c;
+        if (__ballot(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[j][r] *= alpha;
+            m = mn;
+        }
+        // (a row that has seen no key yet keeps m = -inf: weights 0)
+        const float mu = m == -INFINITY ? 0.f : m - C::BIAS;
+#pragma unroll
+        for (int kt = 0; kt < KT32; kt++) l += weights(kt, mu);
+        if constexpr (C::KF) {
+            // weights take over the values' powers of two, less the largest power that keeps them all within range: the
+            // outputs carry that one
+            int low = ve;
+#pragma unroll
+            for (int kt = 0; kt < KT32; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    low = min(low, s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
+            if (miss_here != 0 || k0 + BK - 1 > lim0) {  // (only of values that it sees)
+                asm volatile("");
+                low = ve;
 #pragma unroll
                 for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
                     for (int r = 0; r < 16; r++)
-                        if (32 * kt + 8 * (r >> 2) + (r & 3) > last) s[kt][r] = -INFINITY;
+                        low = min(low, s[kt][r] > 0.f ? s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)] : 100);
             }
-            if (miss != 0) {
-#pragma unroll
-                for (int kt = 0; kt < KT32; kt++) {
-                    const unsigned gone = (unsigned)(miss >> (32 * kt)) >> (4 * h);
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (gone >> (8 * (r >> 2) + (r & 3)) & 1) s[kt][r] = -INFINITY;
-                }
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int kt = 0; kt < KT32; kt++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
-            mx = max_xor32(mx) * c;
-            if (__ballot(mx > m)) {
-                const float mn = fmaxf(m, mx);
-                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-                l *= alpha;
+            low = min(low, __float_as_int(xor32(__int_as_float(low), lane)));
+            if (__ballot(low < ve)) {
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) o[j][r] *= alpha;
-                m = mn;
+                    for (int r = 0; r < 16; r++) o[j][r] = ldexpf(o[j][r], low - ve);
+                ve = low;
             }
-            // (a row that has seen no key yet keeps m = -inf: weights 0)
-            const float mu = m == -INFINITY ? 0.f : m - C::BIAS;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], c, -mu));
-                    sum[r & 3] += s[kt][r];
-                }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);  // this lane's half of the keys
+                for (int r = 0; r < 16; r++)
+                    s[kt][r] = ldexpf(s[kt][r], ve - s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
         }
-        stage_store(vbuf, true);
-        if (masked && clean(k0, miss)) s_bad = tile;
-        if (tile + 1 < t1) stage_load(tile + 1, p.kp, pg0, pg1, pg2, pg3);
-        __syncthreads();
-        const bool bad = masked && s_bad == tile;
-        if (work) {
 #pragma unroll
-            for (int kt = 0; kt < KT32; kt++)
-#pragma unroll
-                for (int k2 = 0; k2 < 2; k2++) {
-                    if (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // one step's planes at a time: registers
-                    unsigned u[4][NQ];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) split2<C::F16, NQ>(s[kt][8 * k2 + 2 * i], s[kt][8 * k2 + 2 * i + 1], u[i]);
-                    u32x4 pf[NQ];
-#pragma unroll
-                    for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
-#pragma unroll
-                    for (int jt = 0; jt < NJ; jt++)
-#pragma unroll
-                        for (int j = 0; j < NK; j++) {
-                            const char* a = vbuf + j * C::PLANE + (vaddr ^ (jt * 64)) + (32 * kt + 16 * k2) * (HD * 2);
-                            typedef __attribute__((address_space(3))) shortx4 lds4;
-                            const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a);
-                            const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(a + 8 * HD * 2));
-                            const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-                            const u32x4 vf = quad(x.x, x.y, y.x, y.y);
-#pragma unroll
-                            for (int i = 0; i < NQ; i++)
-                                if (i + j < C::DEPTH) o[jt] = E::mac(vf, pf[i], o[jt]);
-                        }
-                }
-            if (__builtin_expect(bad, 0)) {
-                // the values that were left out: their weights are positive, so that each is its own contribution
+        for (int kt = 0; kt < KT32; kt++) products(kt);
+        if (__builtin_expect(bad, 0)) {
+            // the values that were left out: their weights are positive, so that each is its own contribution
 #pragma unroll 1
-                for (int key = 0; key < BK && k0 + key < kend; key++) {
-                    const int page = __builtin_amdgcn_readfirstlane(page_of_row(p.table, p.seqs, p.max_pages, p.pages, p.shift, t.seq, k0 + key));
-                    if (page < 0) continue;
-                    const KT* v = (const KT*)p.vp + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((k0 + key) & pmask)) * HD + 4 * h;
-                    const bool seen = k0 + key <= lim;
+            for (int key = 0; key < BK && k0 + key < kend; key++) {
+                const int page = __builtin_amdgcn_readfirstlane(page_of_row(p.table, p.seqs, p.max_pages, p.pages, p.shift, t.seq, k0 + key));
+                if (page < 0) continue;
+                const KT* v = (const KT*)p.vp + ((((size_t)page * p.kv_heads + kvh) << p.shift) + ((k0 + key) & pmask)) * HD + 4 * h;
+                const bool seen = k0 + key <= lim;
 #pragma unroll
-                    for (int j = 0; j < NJ; j++)
+                for (int j = 0; j < NJ; j++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const float x = to_float(v[32 * j + 8 * (r >> 2) + (r & 3)]);
-                            if (seen && !(fabsf(x) < INFINITY)) o[j][r] += x;
-                            if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // few loads at a time: registers
-                        }
-                }
+                    for (int r = 0; r < 16; r++) {
+                        const float x = to_float(v[32 * j + 8 * (r >> 2) + (r & 3)]);
+                        if (seen && !(fabsf(x) < INFINITY)) o[j][r] += x;
+                        if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // few loads at a time: registers
+                    }
             }
         }
     }
     l = sum_xor32(l);
 
     if (!mine) return;
+    if constexpr (C::KF) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[j][r] = ldexpf(o[j][r], -ve);
+    }
     if (t.splits == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         QT* out = (QT*)p.out + qrow;
@@ -649,15 +846,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
     const int tid = threadIdx.x, lane = tid & 63, lq = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % p.kv_heads;
-    Task t;
-    if (!find_task<16, false>(p, blockIdx.x / p.kv_heads, &t)) return;
+    Task found;
+    if (!find_task<16, false>(p, blockIdx.x / p.kv_heads, &found)) return;
+    const Task t = settled(found);
     const int row = t.r0 + lq, packed = t.r0 + t.rows;
     const bool mine = row < packed;
     const int tok = mine ? row / p.group : 0, head = kvh * p.group + (mine ? row - tok * p.group : 0);
     const size_t qrow = ((size_t)(t.first + tok) * p.heads + head) * HD;
-    const long long cap = (long long)p.max_pages << p.shift;
-    auto last_key = [&](int r) { return t.units == 0 ? -1 : (int)(t.at + r / p.group < cap ? t.at + r / p.group : cap - 1); };
-    const int lim = mine ? last_key(row) : -1, lim0 = last_key(t.r0), kend = last_key(packed - 1) + 1;
+    const int lim = mine ? last_key(p, t, row) : -1;
+    const int lim0 = uniform(last_key(p, t, t.r0)), kend = uniform(last_key(p, t, packed - 1)) + 1;
     const int t0 = t.split * t.per * 4 + wave, t1 = min((t.split + 1) * t.per * 4, (kend + 31) / 32);
 
     const TableRow table = table_row(p, t.seq);
@@ -727,7 +924,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[s][i]));
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[s][i]) < INFINITY ? fabsf(v[s][i]) : 0.f);
             top = max_xor32(fmaxf(top, xor16(top, lane)));
             const int e = fp16_shift(top);
             c = ldexpf(c, -e);
@@ -740,7 +937,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
         for (int s = 0; s < KS; s++) {
             unsigned u[4][NQ];
 #pragma unroll
-            for (int i = 0; i < 4; i++) split2<C::F16, NQ>(v[s][2 * i], v[s][2 * i + 1], u[i]);
+            for (int i = 0; i < 4; i++) split2<C::F16, NQ, true>(v[s][2 * i], v[s][2 * i + 1], u[i]);
 #pragma unroll
             for (int n = 0; n < NQ; n++) qf[n][s] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
         }
@@ -786,6 +983,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
         const int next = tile + kWaves;
         load_k(next, pn0, pn1);  // (past the end: rows of no page, not used)
         if (masked) {
+            asm volatile("");  // (a branch: few tiles have hidden keys)
             const int last = lim - k0 - 4 * g;
             const unsigned gone = miss >> (4 * g);
 #pragma unroll
@@ -862,7 +1060,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
             {
                 unsigned u[4][NQ];
 #pragma unroll
-                for (int i = 0; i < 4; i++) split2<C::F16, NQ>(s[i >> 1][2 * (i & 1)], s[i >> 1][2 * (i & 1) + 1], u[i]);
+                for (int i = 0; i < 4; i++) split2<C::F16, NQ, false>(s[i >> 1][2 * (i & 1)], s[i >> 1][2 * (i & 1) + 1], u[i]);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
             }
@@ -949,8 +1147,10 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
     const int kvh = b % p.kv_heads;
     b /= p.kv_heads;
     const int r0 = 16 * (b % (ROWS / 16));
-    Task t;
-    if (!find_task<ROWS, true>(p, b / (ROWS / 16), &t) || t.splits == 1) return;
+    Task found;
+    if (!find_task<ROWS, true>(p, b / (ROWS / 16), &found)) return;
+    const Task t = settled(found);
+    if (t.splits == 1) return;
     const int rows = min(t.rows - r0, 16);
     if (rows <= 0) return;
     int share = 1;  // groups of a row
@@ -986,10 +1186,11 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
 
 // ---- host side ----------------------------------------------------------------------------------------------
 
-// A kernel's share of a call: tasks at most, and how many to cut the keys for (0: none).
+// A kernel's share of a call: its tiles at most, and how many tasks to cut their keys into (0: none; two more per tile
+// for what rounding makes of it).
 struct Part {
     int tiles = 0, target = 0;
-    int tasks() const { return tiles + target; }
+    int tasks() const { return target ? target + 2 * tiles + 1 : tiles; }
     size_t bytes(const ar_pages* p, int rows) const {
         return target ? (size_t)tasks() * p->kv_heads * rows * ((size_t)p->head_dim * 4 + 8) : 0;
     }
@@ -1006,10 +1207,13 @@ struct Plan {
 constexpr int kFewRows = 64, kMaxSplitChunks = 1024;
 
 // Tasks to cut the keys for: `per_cu` blocks a CU over all KV heads, unless the tiles alone are several times that.
-int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu) {
+int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu, int unit) {
     if (tiles * p->kv_heads >= 3LL * per_cu * ctx->num_cus || n > kMaxSplitChunks) return 0;
-    if ((long long)p->max_pages * p->page_rows <= kUnit) return 0;
-    return std::max(1, per_cu * ctx->num_cus / p->kv_heads);
+    if ((long long)p->max_pages * p->page_rows <= unit) return 0;  // (one split of any sequence)
+    // (a chunk's last split is a task of its own, so that there may be `tiles` more; and no more than units)
+    const long long cap = (long long)p->max_pages * p->page_rows;
+    const long long want = std::min((long long)per_cu * ctx->num_cus / p->kv_heads - tiles, std::max(tiles, 1LL) * ((cap + unit - 1) / unit));
+    return (int)std::max(1LL, want);
 }
 
 int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int heads, Plan* out) {
@@ -1017,17 +1221,18 @@ int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int he
     AR_CHECK_ARG(packed <= 1 << 30 && (packed / 16 + c->n) * p->kv_heads <= 1 << 30, "paged attention: %d rows of %d heads are too many",
                  c->rows, heads);
     Plan a;
-    const int few_cu = p->dtype == AR_DTYPE_F32 ? 2 : 3;
+    // (fp32 rows keep twice the bytes in flight: one block a CU was enough; 16-bit caches and tiles: two)
+    const int few_cu = p->dtype == AR_DTYPE_F32 ? 1 : 2, tile_cu = 2;
     if (!c->start || packed <= 32LL * c->n) {
         a.few_rows = 0x7fffffff;
         a.few.tiles = (int)(c->start ? packed / 16 + c->n : c->n * ((group + 15) / 16));
-        a.few.target = target_of(ctx, p, std::max<long long>(c->n, packed / 16), c->n, few_cu);
+        a.few.target = target_of(ctx, p, std::max<long long>(c->n, packed / 16), c->n, few_cu, kUnit<16>);
     } else {
         a.tile.tiles = (int)(packed / 128 + c->n);
-        a.tile.target = target_of(ctx, p, packed / 128, c->n, 2);
+        a.tile.target = target_of(ctx, p, packed / 128, c->n, tile_cu, kUnit<128>);
         if (c->n > 1) {
             a.few_rows = kFewRows;
-            a.few.target = target_of(ctx, p, 0, c->n, few_cu);
+            a.few.target = target_of(ctx, p, 0, c->n, few_cu, kUnit<16>);
             a.few.tiles = (int)(a.few.target ? std::min(packed / 16 + c->n, kFewRows / 16LL * c->n) : packed / 16 + c->n);
         }
     }
