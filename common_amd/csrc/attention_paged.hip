@@ -28,6 +28,14 @@ typedef short shortx4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ u32x4 quad(unsigned a, unsigned b, unsigned c, unsigned d) { return u32x4{a, b, c, d}; }
 
+// One kernel's share of a call.
+struct PartArgs {
+    int tiles, tasks;     // at most
+    int target;           // how many tasks to cut the keys for (0: a tile is a task)
+    float* part;          // [tasks][kv_heads][tile rows][hd] unnormalised outputs of splits, and (m, l) of each
+    float2* part_ml;
+};
+
 struct PagedParams {
     const void* q;
     void* out;
@@ -36,9 +44,7 @@ struct PagedParams {
     int heads, kv_heads, group, seqs, max_pages, pages, shift, n, rows;
     float scale;          // log2(e) / sqrt(head_dim)
     int few_rows;         // chunks of at most this many packed rows are the few-row kernel's
-    int tasks, target;    // tasks of the launch at most; how many to cut the keys for (0: whole rows)
-    float* part;          // [tasks][kv_heads][tile rows][hd] unnormalised outputs of splits, and (m, l) of each
-    float2* part_ml;
+    PartArgs few, tile;
 };
 
 // 16-bit element of the matrix units: bf16, or fp16 for fp16 caches.
@@ -171,8 +177,8 @@ struct Shape {
 
 // ---- what a block works on --------------------------------------------------------------------------------------
 // Tasks are the tiles of ROWS packed rows of every chunk.  Where there are enough of them to fill the GPU, a tile is a task
-// (p.target 0): the block's slot is searched among the chunks, 64 at a time.  Otherwise every block adds up what all
-// chunks' tiles see, so that splits of `per` units of kUnit<ROWS> keys make about p.target tasks of equal length whatever
+// (target 0): the block's slot is searched among the chunks, 64 at a time.  Otherwise every block adds up what all
+// chunks' tiles see, so that splits of `per` units of kUnit<ROWS> keys make about `target` tasks of equal length whatever
 // the lengths of the sequences are, and finds its task in their order.  In a chunk of several tiles, tile j's tasks begin
 // at floor(S(j) / L) + 2 j, with L keys in a split and S(j) the keys that the tiles before j see, from above and in closed
 // form: at least as many as its splits, and found without a sum over tiles; those past its splits are empty.
@@ -245,9 +251,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 // for itself.
 template <int ROWS, bool MERGE>
 __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task* t) {
+    const int target = ROWS == 16 ? p.few.target : p.tile.target;
     const int lane = threadIdx.x & 63;
     int tile = 0;
-    if (p.target == 0) {
+    if (target == 0) {
         const int per_chunk = (p.group + ROWS - 1) / ROWS;
         const int chunk = !p.start ? index / per_chunk : chunk_search(p.n, 64, [&](int i, int k, int len) {
             const bool below = (long long)lane * k < len && chunk_slot(p.start[i + lane * k], i + lane * k, p.group, ROWS) <= index;
@@ -274,7 +281,7 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) keys += __shfl_xor(keys, d);
-        const int per = (int)fmax(1., fmin(ceil(keys / ((double)p.target * kUnit<ROWS>)), 1 << 24));
+        const int per = (int)fmax(1., fmin(ceil(keys / ((double)target * kUnit<ROWS>)), 1 << 24));
         const double inv = 1. / ((double)per * kUnit<ROWS>);
         int tasks = 0, tiles = 0;  // before this round's chunks
         bool found = false;
@@ -384,20 +391,26 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 template <int HD, typename QT, typename KT>
-__global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p) {
+struct TileSpace {
+    typedef Shape<HD, QT, KT> C;
+    char lds[4 * C::TILE];      // keys and values of a tile and of the next
+    int s_exp[2][2][C::BK];     // fp32 caches: powers of two that they carry
+    int s_bad[2];
+};
+
+template <int HD, typename QT, typename KT>
+__device__ __forceinline__ void tile_block(const PagedParams& p, int index, int kvh, TileSpace<HD, QT, KT>& space) {
     typedef Shape<HD, QT, KT> C;
     typedef Elem<C::F16> E;
     constexpr int NQ = C::NQ, NK = C::NK, BK = C::BK, KT32 = BK / 32, NJ = HD / 32, KS = HD / 16;
-    __shared__ __attribute__((aligned(16))) char lds[4 * C::TILE];  // keys and values of a tile and of the next
-    __shared__ __attribute__((aligned(16))) int s_exp[2][2][BK];    // fp32 caches: powers of two that they carry
-    __shared__ int s_bad[2];
+    char* const lds = space.lds;
+    int (*const s_exp)[2][BK] = space.s_exp;
+    int* const s_bad = space.s_bad;
 
     const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // KV head fastest (8 of them: one to an XCD, whose L2 then holds that head's rows), later rows, with more keys, first
-    const int kvh = blockIdx.x % p.kv_heads;
     Task found;
-    if (!find_task<C::ROWS, false>(p, p.tasks - 1 - (int)(blockIdx.x / p.kv_heads), &found)) return;
+    if (!find_task<C::ROWS, false>(p, index, &found)) return;
     const Task t = settled(found);
 
     const int row = t.r0 + 32 * wave + lq, packed = t.r0 + t.rows;  // row: packed, in the chunk
@@ -819,8 +832,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p)
         for (int j = 0; j < NJ; j++)
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
-                store4(p.part + at * HD + 32 * j + 2 * r + 4 * h, o[j][r], o[j][r + 1], o[j][r + 2], o[j][r + 3]);
-        if (h == 0) p.part_ml[at] = make_float2(m, l);
+                store4(p.tile.part + at * HD + 32 * j + 2 * r + 4 * h, o[j][r], o[j][r + 1], o[j][r + 2], o[j][r + 3]);
+        if (h == 0) p.tile.part_ml[at] = make_float2(m, l);
     }
 }
 
@@ -833,21 +846,27 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tiles_kernel(PagedParams p)
 // fp32 ones do not: v_mfma_f32_16x16x4_f32 wants one value of a key per lane, and output row i of tile (a, j) is dim
 // 64 a + 4 i + j, so that 16 bytes of a value row feed four tiles.  Of the next tile, keys are loaded when this one's
 // scores are done and values when its own are in LDS (or used).
+template <int HD>
+struct FewSpace {
+    char lds[kWaves * 32 * HD * 2];  // values, later the wavefronts' outputs
+    float s_m[kWaves][16], s_l[kWaves][16];
+};
+
 template <int HD, typename QT, typename KT>
-__global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
+__device__ __forceinline__ void few_block(const PagedParams& p, int index, int kvh, FewSpace<HD>& space) {
     typedef Shape<HD, QT, KT> C;
     typedef Elem<C::F16> E;
     constexpr bool KF = C::KF;
     constexpr int NQ = C::NQ, NJ = HD / 16, KS = HD / 32, QC = HD / 16, JJ = HD / 64;
     constexpr int ROW = HD * (int)sizeof(KT), UNITS = 32 * C::CPR / 64, VBYTES = 32 * HD * 2;
-    __shared__ __attribute__((aligned(16))) char lds[kWaves * VBYTES];  // values, later the wavefronts' outputs
-    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+    char* const lds = space.lds;
+    float (*const s_m)[16] = space.s_m;
+    float (*const s_l)[16] = space.s_l;
 
     const int tid = threadIdx.x, lane = tid & 63, lq = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x % p.kv_heads;
     Task found;
-    if (!find_task<16, false>(p, blockIdx.x / p.kv_heads, &found)) return;
+    if (!find_task<16, false>(p, index, &found)) return;
     const Task t = settled(found);
     const int row = t.r0 + lq, packed = t.r0 + t.rows;
     const bool mine = row < packed;
@@ -1130,22 +1149,35 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few_kernel(PagedParams p) {
             v[i] = ((a[0] + a[NJ * 256]) + (a[2 * NJ * 256] + a[3 * NJ * 256])) * inv;
         }
         const int d = KF ? 64 * q + 4 * (4 * g + wave) : 16 * (q + NJ / 4 * wave) + 4 * g;
-        if (t.splits > 1) store4(p.part + at * HD + d, v[0], v[1], v[2], v[3]);
+        if (t.splits > 1) store4(p.few.part + at * HD + d, v[0], v[1], v[2], v[3]);
         else store4((QT*)p.out + qrow + d, v[0], v[1], v[2], v[3]);
     }
-    if (t.splits > 1 && wave == 0 && g == 0) p.part_ml[at] = make_float2(mm, l);
+    if (t.splits > 1 && wave == 0 && g == 0) p.few.part_ml[at] = make_float2(mm, l);
+}
+
+// ---- both in one launch -------------------------------------------------------------------------------------------
+// PARTS: 1 few rows, 2 tiles, 3 both (blocks of tiles first).  KV head fastest (8 of them: one to an XCD, whose L2 then
+// holds that head's rows); tiles from the last, with the most keys, on.
+template <int HD, typename QT, typename KT, int PARTS>
+__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedParams p) {
+    union Space {
+        TileSpace<HD, QT, KT> tile;
+        FewSpace<HD> few;
+    };
+    __shared__ __attribute__((aligned(16))) char space[PARTS == 1 ? sizeof(FewSpace<HD>) : sizeof(Space)];
+    const int kvh = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads;
+    if (PARTS == 2 || (PARTS == 3 && b < p.tile.tasks))
+        tile_block<HD, QT, KT>(p, p.tile.tasks - 1 - b, kvh, *reinterpret_cast<TileSpace<HD, QT, KT>*>(space));
+    else if (PARTS & 1)
+        few_block<HD, QT, KT>(p, b - (PARTS == 3 ? p.tile.tasks : 0), kvh, *reinterpret_cast<FewSpace<HD>*>(space));
 }
 
 // ---- the splits of a row, in a fixed order ------------------------------------------------------------------------
 // A block takes 16 rows of a tile; where a tile has fewer, several groups of HD / 4 lanes share a row's splits.
 template <int HD, typename QT, int ROWS>
-__global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
+__device__ __forceinline__ void merge_block(const PagedParams& p, int b, int kvh, float (*s_o)[HD], float* s_l) {
     constexpr int LPR = HD / 4, NG = 512 / LPR;
-    __shared__ __attribute__((aligned(16))) float s_o[NG][HD];
-    __shared__ float s_l[NG];
-    int b = blockIdx.x;
-    const int kvh = b % p.kv_heads;
-    b /= p.kv_heads;
+    const PartArgs& a = ROWS == 16 ? p.few : p.tile;
     const int r0 = 16 * (b % (ROWS / 16));
     Task found;
     if (!find_task<ROWS, true>(p, b / (ROWS / 16), &found)) return;
@@ -1158,14 +1190,14 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
     const int group = threadIdx.x / LPR, col = threadIdx.x % LPR, r = group / share, sub = group % share;
     const size_t step = (size_t)p.kv_heads * ROWS, at = ((size_t)t.base * p.kv_heads + kvh) * ROWS + r0 + min(r, rows - 1);
     float m = -INFINITY, l = 0.f;
-    for (int s = col; s < t.splits; s += LPR) m = fmaxf(m, p.part_ml[at + s * step].x);
+    for (int s = col; s < t.splits; s += LPR) m = fmaxf(m, a.part_ml[at + s * step].x);
 #pragma unroll
     for (int d = 1; d < LPR; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int s = sub; s < t.splits; s += share) {
-        const float2 ml = p.part_ml[at + s * step];
-        const float4 v = *reinterpret_cast<const float4*>(p.part + (at + s * step) * HD + 4 * col);
+        const float2 ml = a.part_ml[at + s * step];
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (at + s * step) * HD + 4 * col);
         const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // (no key seen: zeros)
         l = fmaf(ml.y, f, l);
         o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
@@ -1182,6 +1214,15 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int row = t.r0 + r0 + r, tok = row / p.group, head = kvh * p.group + row - tok * p.group;
     store4((QT*)p.out + ((size_t)(t.first + tok) * p.heads + head) * HD + 4 * col, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+template <int HD, typename QT>
+__global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
+    __shared__ __attribute__((aligned(16))) float s_o[512 / (HD / 4)][HD];
+    __shared__ float s_l[512 / (HD / 4)];
+    const int kvh = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads, tiles = p.tile.target ? 8 * p.tile.tiles : 0;
+    if (b < tiles) merge_block<HD, QT, 128>(p, b, kvh, s_o, s_l);
+    else merge_block<HD, QT, 16>(p, b - tiles, kvh, s_o, s_l);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
@@ -1245,28 +1286,19 @@ size_t plan_bytes(const ar_pages* p, const Plan& a) { return std::max<size_t>(16
 template <int HD, typename QT, typename KT>
 int launch_plan(const ar_pages* pages, const Plan& a, PagedParams p, char* work, hipStream_t st) {
     auto part = [&](const Part& x, int rows, char* at) {
-        p.tasks = x.tasks();
-        p.target = x.target;
-        p.part = (float*)at;
-        p.part_ml = (float2*)(at + (size_t)x.tasks() * p.kv_heads * rows * HD * 4);
+        return PartArgs{x.tiles, x.tasks(), x.target, (float*)at, (float2*)(at + (size_t)x.tasks() * p.kv_heads * rows * HD * 4)};
     };
-    if (a.tile.tiles) {
-        part(a.tile, 128, work + a.few.bytes(pages, 16));
-        hipLaunchKernelGGL((paged_tiles_kernel<HD, QT, KT>), dim3((unsigned)p.tasks * p.kv_heads), dim3(kThreads), 0, st, p);
+    p.few = part(a.few, 16, work);
+    p.tile = part(a.tile, 128, work + a.few.bytes(pages, 16));
+    const dim3 grid((unsigned)(p.few.tasks + p.tile.tasks) * p.kv_heads), block(kThreads);
+    if (!p.tile.tasks) hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 1>), grid, block, 0, st, p);
+    else if (!p.few.tasks) hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 2>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 3>), grid, block, 0, st, p);
+    AR_LAUNCH_CHECK();
+    const int merges = (p.tile.target ? 8 * p.tile.tiles : 0) + (p.few.target ? p.few.tiles : 0);
+    if (merges) {
+        hipLaunchKernelGGL((paged_merge_kernel<HD, QT>), dim3((unsigned)merges * p.kv_heads), dim3(512), 0, st, p);
         AR_LAUNCH_CHECK();
-        if (p.target) {
-            hipLaunchKernelGGL((paged_merge_kernel<HD, QT, 128>), dim3((unsigned)a.tile.tiles * 8 * p.kv_heads), dim3(512), 0, st, p);
-            AR_LAUNCH_CHECK();
-        }
-    }
-    if (a.few.tiles) {
-        part(a.few, 16, work);
-        hipLaunchKernelGGL((paged_few_kernel<HD, QT, KT>), dim3((unsigned)p.tasks * p.kv_heads), dim3(kThreads), 0, st, p);
-        AR_LAUNCH_CHECK();
-        if (p.target) {
-            hipLaunchKernelGGL((paged_merge_kernel<HD, QT, 16>), dim3((unsigned)a.few.tiles * p.kv_heads), dim3(512), 0, st, p);
-            AR_LAUNCH_CHECK();
-        }
     }
     return AR_HIP_OK;
 }

@@ -7,9 +7,9 @@ namespace {
 constexpr int kMaxEntries = 4096;  // chunks / entries of one table call: their state lies in one block's LDS
 
 // ---- page copies -----------------------------------------------------------------------------------
-// Bound by HBM, each byte read and written once.  A block moves pieces of 32 KB: 256 threads x four 16-byte loads
-// in flight before their stores, so 8 blocks on a CU keep 128 KB in flight.
-constexpr int kCopyThreads = 256, kCopyUnroll = 4, kPieceBytes = 32768;
+// Bound by HBM, each byte read and written once.  A block moves pieces of 16 KB: 256 threads x four 16-byte loads in
+// flight before their stores, so 8 blocks on a CU keep 128 KB in flight.
+constexpr int kCopyThreads = 256, kCopyUnroll = 4, kPieceBytes = 16384;
 
 struct CopyParams {
     const char *sk, *sv;

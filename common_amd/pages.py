@@ -79,7 +79,7 @@ class PagedCache:
         self.ctx, self.dtype = ctx, dtype
         self.layers, self.pages, self.kv_heads, self.head_size = layers, pages, kv_heads, head_size
         self.seqs, self.max_pages, self.page_rows = seqs, max_pages, page_rows
-        self._own, self._work, self._need = [], None, {}
+        self._own, self._work, self._need = [], None, {}  # (_need: work bytes by kind of call)
 
         def take(buf, nbytes, fill):
             if buf is not None or nbytes == 0:
@@ -114,21 +114,21 @@ class PagedCache:
     def __exit__(self, *exc):
         self.close()
 
-    def _scratch(self, key, query):
-        """The cache's work space, grown to what `query` says this kind of call needs."""
-        need = self._need.get(key)
-        if need is None:
-            b = ctypes.c_size_t()
-            check(query(ctypes.byref(b)))
-            need = self._need[key] = max(b.value, 16)
+    def _scratch(self, need):
+        """The cache's work space, grown to `need` bytes."""
         if self._work is None or self._work.nbytes < need:
             if self._work is not None:
                 self._work.free()
+                self._work = None
             self._work = self.ctx.allocate(need)
         return self._work
 
     def _table_scratch(self, n):
-        return self._scratch(n, lambda b: lib().ar_hip_pages_work(self.ref, n, b))
+        if n not in self._need:
+            b = ctypes.c_size_t()
+            check(lib().ar_hip_pages_work(self.ref, n, ctypes.byref(b)))
+            self._need[n] = b.value
+        return self._scratch(self._need[n])
 
     def grow(self, chunks: Chunks, missing=None):
         """Room for the chunks' rows at their sequences' ends; fills chunks.at (ar_hip_pages_grow)."""
@@ -164,7 +164,11 @@ class PagedCache:
 
     def attention(self, layer: int, chunks: Chunks, q, out, heads: int, act_dtype: int = DTYPE_F32):
         """Causal attention of the chunks' rows over their sequences' pages (ar_hip_attention_paged)."""
-        w = self._scratch((chunks.n, chunks.rows, chunks.start is None, heads),
-                          lambda b: lib().ar_hip_attention_paged_work(self.ctx.handle, self.ref, chunks.ref, heads, b))
+        key = (chunks.n, chunks.rows, chunks.start is None, heads)
+        if key not in self._need:
+            b = ctypes.c_size_t()
+            check(lib().ar_hip_attention_paged_work(self.ctx.handle, self.ref, chunks.ref, heads, ctypes.byref(b)))
+            self._need[key] = b.value
+        w = self._scratch(self._need[key])
         check(lib().ar_hip_attention_paged(self.ctx.handle, self.ref, layer, chunks.ref, _ptr(q), act_dtype, heads,
                                            _ptr(out), w.ptr, w.nbytes))
