@@ -180,7 +180,7 @@ struct Shape {
 // (target 0): the block's slot is searched among the chunks, 64 at a time.  Otherwise every block adds up what all
 // chunks' tiles see, so that splits of `per` units of kUnit<ROWS> keys make about `target` tasks of equal length whatever
 // the lengths of the sequences are, and finds its task in their order.  In a chunk of several tiles, tile j's tasks begin
-// at floor(S(j) / L) + 2 j, with L keys in a split and S(j) the keys that the tiles before j see, from above and in closed
+// at floor(S(j) / L) + j, with L keys in a split and S(j) the keys that the tiles before j see, from above and in closed
 // form: at least as many as its splits, and found without a sum over tiles; those past its splits are empty.
 template <int ROWS>
 constexpr int kUnit = ROWS == 16 ? 128 : 64;  // a round of the few-row kernel's wavefronts; the tile kernel's largest key tile
@@ -220,7 +220,7 @@ __device__ __forceinline__ int chunk_tiles(const PagedParams& p, int i, Task* t)
     return (packed + ROWS - 1) / ROWS;
 }
 
-// Keys that tile j of the chunk's n sees; S(j) above; first task of tile j.
+// Keys that tile j of the chunk sees; S(j) above; first task of tile j.
 template <int ROWS>
 __device__ __forceinline__ int tile_end(const PagedParams& p, const Task& c, int j) {
     const int cap = p.max_pages << p.shift, packed = c.count * p.group;
@@ -233,22 +233,23 @@ __device__ __forceinline__ double keys_before(const PagedParams& p, const Task& 
 }
 template <int ROWS>
 __device__ __forceinline__ int first_task(const PagedParams& p, const Task& c, int j, double inv) {
-    return (int)(keys_before<ROWS>(p, c, j) * inv) + 2 * j;
+    return (int)(keys_before<ROWS>(p, c, j) * inv) + j;
 }
 
-// Sum over the wavefront, and of the lanes up to and with this one.
+// Sum over the lanes up to and with this one (row shifts, then row broadcasts).
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int x = __shfl_up(v, d);
-        if (lane >= d) v += x;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
 }
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // Task `index` (MERGE: tile `index` and its first task) -> *t, by one wavefront; every wavefront of a block computes it
-// for itself.
+// for itself, without LDS: it is the first thing that a block waits for.
 template <int ROWS, bool MERGE>
 __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task* t) {
     const int target = ROWS == 16 ? p.few.target : p.tile.target;
@@ -273,15 +274,15 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         // (of up to 64 chunks each lane keeps its own)
         Task c;
         int n = chunk_tiles<ROWS>(p, lane, &c);
-        double keys = keys_before<ROWS>(p, c, n);
+        float keys = n == 1 ? (float)c.units * kUnit<ROWS> : (float)keys_before<ROWS>(p, c, n);
         for (int i = lane + 64; i < p.n; i += 64) {
             Task d;
             const int k = chunk_tiles<ROWS>(p, i, &d);
-            keys += keys_before<ROWS>(p, d, k);
+            keys += k == 1 ? (float)d.units * kUnit<ROWS> : (float)keys_before<ROWS>(p, d, k);
         }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) keys += __shfl_xor(keys, d);
-        const int per = (int)fmax(1., fmin(ceil(keys / ((double)target * kUnit<ROWS>)), 1 << 24));
+        keys = __int_as_float(lane_value(__float_as_int(wave_sum_lane63(keys)), 63));
+        // (a little more than the even share, for the sum's roundings)
+        const int per = (int)fmaxf(1.f, fminf(ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)), 1 << 24));
         const double inv = 1. / ((double)per * kUnit<ROWS>);
         int tasks = 0, tiles = 0;  // before this round's chunks
         bool found = false;
@@ -292,12 +293,12 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
             const unsigned long long m = __ballot((MERGE ? tiles + b : tasks + a) > index);
             if (m) {
                 const int l = __builtin_ctzll(m);
-                t->first = __shfl(c.first, l);
-                t->count = __shfl(c.count, l);
-                t->seq = __shfl(c.seq, l);
-                t->at = __shfl(c.at, l);
-                t->units = __shfl(c.units, l);
-                const int all = __shfl(n, l), a0 = tasks + __shfl(a, l) - __shfl(mine, l), b0 = tiles + __shfl(b, l) - all;
+                t->first = lane_value(c.first, l);
+                t->count = lane_value(c.count, l);
+                t->seq = lane_value(c.seq, l);
+                t->at = lane_value(c.at, l);
+                t->units = lane_value(c.units, l);
+                const int all = lane_value(n, l), a0 = tasks + lane_value(a, l) - lane_value(mine, l), b0 = tiles + lane_value(b, l) - all;
                 const int q = index - (MERGE ? b0 : a0);
                 if (MERGE || all == 1) {
                     tile = MERGE ? q : 0;
@@ -316,8 +317,8 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
                 t->base = a0 + begin;
                 found = true;
             }
-            tasks += __shfl(a, 63);
-            tiles += __shfl(b, 63);
+            tasks += lane_value(a, 63);
+            tiles += lane_value(b, 63);
         }
         if (!found || t->split >= t->splits) return false;
         t->per = per;
@@ -1182,7 +1183,8 @@ __device__ __forceinline__ void merge_block(const PagedParams& p, int b, int kvh
     Task found;
     if (!find_task<ROWS, true>(p, b / (ROWS / 16), &found)) return;
     const Task t = settled(found);
-    if (t.splits == 1) return;
+    // (chunks whose starts are not in order may have more tasks than there is space for: they are not all computed)
+    if (t.splits == 1 || t.base < 0 || t.base + t.splits > a.tasks) return;
     const int rows = min(t.rows - r0, 16);
     if (rows <= 0) return;
     int share = 1;  // groups of a row
@@ -1227,11 +1229,11 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
 
 // ---- host side ----------------------------------------------------------------------------------------------
 
-// A kernel's share of a call: its tiles at most, and how many tasks to cut their keys into (0: none; two more per tile
+// A kernel's share of a call: its tiles at most, and how many tasks to cut their keys into (0: none; one more per tile
 // for what rounding makes of it).
 struct Part {
     int tiles = 0, target = 0;
-    int tasks() const { return target ? target + 2 * tiles + 1 : tiles; }
+    int tasks() const { return target ? target + tiles + 1 : tiles; }
     size_t bytes(const ar_pages* p, int rows) const {
         return target ? (size_t)tasks() * p->kv_heads * rows * ((size_t)p->head_dim * 4 + 8) : 0;
     }
@@ -1251,9 +1253,10 @@ constexpr int kFewRows = 64, kMaxSplitChunks = 1024;
 int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu, int unit) {
     if (tiles * p->kv_heads >= 3LL * per_cu * ctx->num_cus || n > kMaxSplitChunks) return 0;
     if ((long long)p->max_pages * p->page_rows <= unit) return 0;  // (one split of any sequence)
-    // (a chunk's last split is a task of its own, so that there may be `tiles` more; and no more than units)
+    // (a tile's last split is a task of its own, so that there may be `tiles` more; and no more than units)
     const long long cap = (long long)p->max_pages * p->page_rows;
-    const long long want = std::min((long long)per_cu * ctx->num_cus / p->kv_heads - tiles, std::max(tiles, 1LL) * ((cap + unit - 1) / unit));
+    const long long blocks = (long long)per_cu * ctx->num_cus / p->kv_heads - tiles;
+    const long long want = std::min(blocks, std::max(tiles, 1LL) * ((cap + unit - 1) / unit));
     return (int)std::max(1LL, want);
 }
 
