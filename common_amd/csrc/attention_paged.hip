@@ -1247,11 +1247,12 @@ struct Plan {
     Part few, tile;
 };
 
-constexpr int kFewRows = 64, kMaxSplitChunks = 1024;
+constexpr int kFewRows = 16, kMaxSplitChunks = 1024;
 
-// Tasks to cut the keys for: `per_cu` blocks a CU over all KV heads, unless the tiles alone are several times that.
+// Tasks to cut the keys for: `per_cu` blocks a CU over all KV heads, the number that is resident at once, unless the tiles
+// alone are as many (1,024 tokens of three sequences, 537 tiles for 512 blocks: whole tiles 609 us, cut ones 632).
 int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu, int unit) {
-    if (tiles * p->kv_heads >= 3LL * per_cu * ctx->num_cus || n > kMaxSplitChunks) return 0;
+    if (tiles * p->kv_heads >= (long long)per_cu * ctx->num_cus || n > kMaxSplitChunks) return 0;
     if ((long long)p->max_pages * p->page_rows <= unit) return 0;  // (one split of any sequence)
     // (a tile's last split is a task of its own, so that there may be `tiles` more; and no more than units)
     const long long cap = (long long)p->max_pages * p->page_rows;
