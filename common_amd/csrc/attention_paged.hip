@@ -198,7 +198,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // The table is read with scalar loads: nothing writes it while these kernels run.
 typedef const __attribute__((address_space(4))) int* TableRow;
 __device__ __forceinline__ TableRow table_row(const PagedParams& p, int seq) {
-    return (TableRow)(uintptr_t)(p.table + (size_t)(seq < 0 ? 0 : seq) * p.max_pages);
+    return (TableRow)(uintptr_t)(p.table + (size_t)(seq < 0 || seq >= p.seqs ? 0 : seq) * p.max_pages);
 }
 
 // Chunk i's rows, sequence and place; the number of its tiles (0: not this kernel's, or i past the last chunk).
@@ -282,8 +282,9 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         }
         keys = __int_as_float(lane_value(__float_as_int(wave_sum_lane63(keys)), 63));
         // (a little more than the even share, for the sum's roundings)
-        const int per = (int)fmaxf(1.f, fminf(ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)), 1 << 24));
-        const double inv = 1. / ((double)per * kUnit<ROWS>);
+        const float share = fmaxf(1.f, ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)));
+        const double inv = 1. / ((double)share * kUnit<ROWS>);
+        const int per = (int)fminf(share, 1 << 24);  // (no chunk has more units)
         int tasks = 0, tiles = 0;  // before this round's chunks
         bool found = false;
         for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
@@ -430,7 +431,8 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
 #pragma unroll
         for (int r = 0; r < 16; r++) o[j][r] = 0.f;
     float m = -INFINITY, l = 0.f;
-    int ve = 100;  // (fp32 caches) the outputs are times 2^ve
+    float wm = 0.f;  // (fp32 caches) the largest weight, times its value row's power of two; the outputs are times 2^ve
+    int ve = 120;
 
     const int t0 = t.split * t.per * (kUnit<128> / BK), t1 = min(t0 + t.per * (kUnit<128> / BK), (kend + BK - 1) / BK);
     const TableRow table = table_row(p, t.seq);
@@ -518,7 +520,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
 #pragma unroll
                 for (int n = 0; n < NK; n++)
                     *reinterpret_cast<u32x4*>(dst + n * C::PLANE) = quad(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
-                if (col == 0) s_exp[odd][values][key] = e;
+                if (col == 0) s_exp[odd][values][key] = -e;
             } else {
                 *reinterpret_cast<u32x4*>(dst) = st[u];
             }
@@ -535,7 +537,6 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                                                     ((col ^ value_swizzle(key)) * 16));
             const bool out = k0 + key >= kend || (miss >> key & 1);
             any |= leave_out<C::F16>(at, out);
-            if (C::KF && out) s_exp[odd][1][key] = 100;
         }
         return any != 0;
     };
@@ -700,7 +701,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                 float mx = largest(0);
                 float sum = weights(0, mu);
                 if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
-                if (!__ballot(!(mx * c <= m + kSlack))) {
+                if (!__ballot(!(fmaf(mx, c, -m) <= kSlack))) {  // (no key seen yet: NaN or infinity)
                     if (NQ > 1) __builtin_amdgcn_s_setprio(1);
                     products(0);
                     if (NQ > 1) __builtin_amdgcn_s_setprio(0);
@@ -719,7 +720,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[kt][r] = ldexpf(s[kt][r], -s_exp[odd][0][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
+                for (int r = 0; r < 16; r++) s[kt][r] = ldexpf(s[kt][r], s_exp[odd][0][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
         }
         if (k0 + BK - 1 > lim0) {  // (the lane's keys are 32 kt + 8 (r / 4) + r % 4, and 4 h)
             asm volatile("");      // (a branch: few tiles have hidden keys)
@@ -747,6 +748,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
             const float mn = fmaxf(m, mx);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= alpha;
+            if (C::KF) wm *= alpha;
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
@@ -758,36 +760,31 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
 #pragma unroll
         for (int kt = 0; kt < KT32; kt++) l += weights(kt, mu);
         if constexpr (C::KF) {
-            // weights take over the values' powers of two, less the largest power that keeps them all within range: the
-            // outputs carry that one
-            int low = ve;
+            // weights take over the values' powers of two, and a power of the row's that brings the largest so far
+            // into [2^3, 2^15]: bits are lost relative to the largest contribution, not to the largest value
+            float top = 0.f;
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    low = min(low, s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
-            if (miss_here != 0 || k0 + BK - 1 > lim0) {  // (only of values that it sees)
-                asm volatile("");
-                low = ve;
-#pragma unroll
-                for (int kt = 0; kt < KT32; kt++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        low = min(low, s[kt][r] > 0.f ? s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)] : 100);
-            }
-            low = min(low, __float_as_int(xor32(__int_as_float(low), lane)));
-            if (__ballot(low < ve)) {
+                for (int r = 0; r < 16; r++) {
+                    s[kt][r] = ldexpf(s[kt][r], s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
+                    top = fmaxf(top, s[kt][r]);
+                }
+            wm = fmaxf(wm, max_xor32(top));
+            const float x = ldexpf(wm, ve);
+            if (__ballot(x > 32768.f || (x < 8.f && ve < 120))) {
+                const int to = min(137 - (int)(__float_as_uint(wm) >> 23), 120);  // the largest to [2^10, 2^11)
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) o[j][r] = ldexpf(o[j][r], low - ve);
-                ve = low;
+                    for (int r = 0; r < 16; r++) o[j][r] = ldexpf(o[j][r], to - ve);
+                ve = to;
             }
+            const float scale = __uint_as_float((unsigned)(ve + 127) << 23);
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    s[kt][r] = ldexpf(s[kt][r], ve - s_exp[odd][1][32 * kt + 8 * (r >> 2) + 4 * h + (r & 3)]);
+                for (int r = 0; r < 16; r++) s[kt][r] *= scale;
         }
 #pragma unroll
         for (int kt = 0; kt < KT32; kt++) products(kt);
@@ -1257,13 +1254,13 @@ int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, 
     // (a tile's last split is a task of its own, so that there may be `tiles` more; and no more than units)
     const long long cap = (long long)p->max_pages * p->page_rows;
     const long long blocks = (long long)per_cu * ctx->num_cus / p->kv_heads - tiles;
-    const long long want = std::min(blocks, std::max(tiles, 1LL) * ((cap + unit - 1) / unit));
+    const long long want = std::min(blocks, std::max<long long>(tiles, n) * ((cap + unit - 1) / unit));
     return (int)std::max(1LL, want);
 }
 
 int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int heads, Plan* out) {
     const long long group = heads / p->kv_heads, packed = (long long)c->rows * group;
-    AR_CHECK_ARG(packed <= 1 << 30 && (packed / 16 + c->n) * p->kv_heads <= 1 << 30, "paged attention: %d rows of %d heads are too many",
+    AR_CHECK_ARG(packed <= 1 << 30 && (packed / 16 + c->n) * p->kv_heads < 1 << 23, "paged attention: %d rows of %d heads are too many",
                  c->rows, heads);
     Plan a;
     // (fp32 rows keep twice the bytes in flight: one block a CU was enough; 16-bit caches and tiles: two)

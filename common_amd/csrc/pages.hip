@@ -467,6 +467,7 @@ int page_check_chunks(const ar_pages* p, const ar_chunks* c, const char* what) {
     AR_CHECK_ARG(c->at, "%s: chunks have no cache rows (at)", what);
     AR_CHECK_ARG(c->n > 0 && c->n <= 1 << 20, "%s: %d chunks not in [1,2^20]", what, c->n);
     AR_CHECK_ARG(c->rows >= 0, "%s: negative row count", what);
+    AR_CHECK_ARG(c->rows <= 1 << 22, "%s: %d rows are more than 2^22", what, c->rows);
     AR_CHECK_ARG(c->start || c->rows >= c->n, "%s: %d rows for %d chunks of one row", what, c->rows, c->n);
     AR_CHECK_ARG(c->seq || c->n <= p->seqs, "%s: %d chunks for %d sequences", what, c->n, p->seqs);
     return AR_HIP_OK;
@@ -604,9 +605,16 @@ extern "C" int ar_hip_pages_copy(ar_hip_ctx* ctx, const ar_pages* from, const ar
     AR_CHECK_ARG(from->dtype == to->dtype && from->layers == to->layers && from->kv_heads == to->kv_heads &&
                      from->page_rows == to->page_rows && from->head_dim == to->head_dim,
                  "%s: the pools differ in dtype, layers, kv_heads, page_rows or head_dim", what);
-    AR_CHECK_ARG((from->k == to->k) == (from->v == to->v) && from->k != to->v && from->v != to->k,
+    const bool same = from->k == to->k && from->v == to->v;
+    AR_CHECK_ARG(!same || from->pages == to->pages, "%s: one pool with two page counts", what);
+    const size_t page = (size_t)from->layers * from->kv_heads * from->page_rows * from->head_dim * page_elem_bytes(from->dtype);
+    auto overlap = [&](const void* a, int na, const void* b, int nb) {
+        const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+        return x < y + page * nb && y < x + page * na;
+    };
+    AR_CHECK_ARG(same || !(overlap(from->k, from->pages, to->k, to->pages) || overlap(from->v, from->pages, to->v, to->pages) ||
+                           overlap(from->k, from->pages, to->v, to->pages) || overlap(from->v, from->pages, to->k, to->pages)),
                  "%s: the pools share part of their memory", what);
-    AR_CHECK_ARG(from->k != to->k || from->pages == to->pages, "%s: one pool with two page counts", what);
     AR_TRY(check_entries(n, what));
     AR_CHECK_ARG(src && dst, "%s: null page list", what);
     AR_CHECK_ARG(ctx, "ctx is null");
@@ -619,6 +627,6 @@ extern "C" int ar_hip_pages_copy(ar_hip_ctx* ctx, const ar_pages* from, const ar
     c.src = src;
     c.dst = dst;
     c.slots = n;
-    c.same_pool = from->k == to->k;
+    c.same_pool = same;
     return launch_copy(ctx, c);
 }

@@ -11,7 +11,8 @@ No counterpart in the reference (one contiguous cache per model, AttentionFeatur
         cache.write(layer, rows, q, k, v, q_out, heads, rotary)
         cache.attention(layer, rows, q_out, out, heads)
 
-Buffers are anything with a ``ptr`` (``hardware.DeviceBuffer``).  Everything runs on the context's stream.
+Buffers are anything with a ``ptr`` (``hardware.DeviceBuffer``).  Everything runs on the context's stream.  A call that
+needs more work space than any before it allocates it; the space that queued calls still use stays until ``close``.
 """
 from __future__ import annotations
 
@@ -79,7 +80,7 @@ class PagedCache:
         self.ctx, self.dtype = ctx, dtype
         self.layers, self.pages, self.kv_heads, self.head_size = layers, pages, kv_heads, head_size
         self.seqs, self.max_pages, self.page_rows = seqs, max_pages, page_rows
-        self._own, self._work, self._need = [], None, {}  # (_need: work bytes by kind of call)
+        self._own, self._work, self._need = [], [], {}  # (_work: the last is in use; _need: work bytes by kind of call)
 
         def take(buf, nbytes, fill):
             if buf is not None or nbytes == 0:
@@ -100,13 +101,11 @@ class PagedCache:
         self.ref = ctypes.byref(self.raw)
 
     def close(self):
-        """Frees the buffers this cache allocated."""
-        for buf in self._own:
+        """Frees the buffers this cache allocated; calls after it are refused."""
+        for buf in self._own + self._work:
             buf.free()
-        self._own = []
-        if self._work is not None:
-            self._work.free()
-            self._work = None
+        self._own, self._work = [], []
+        self.raw.k = self.raw.v = None
 
     def __enter__(self):
         return self
@@ -115,13 +114,10 @@ class PagedCache:
         self.close()
 
     def _scratch(self, need):
-        """The cache's work space, grown to `need` bytes."""
-        if self._work is None or self._work.nbytes < need:
-            if self._work is not None:
-                self._work.free()
-                self._work = None
-            self._work = self.ctx.allocate(need)
-        return self._work
+        """The cache's work space, of at least `need` bytes."""
+        if not self._work or self._work[-1].nbytes < need:
+            self._work.append(self.ctx.allocate(max(need, 2 * self._work[-1].nbytes if self._work else 0)))
+        return self._work[-1]
 
     def _table_scratch(self, n):
         if n not in self._need:

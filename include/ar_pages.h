@@ -53,7 +53,7 @@ typedef struct ar_chunks {
     int32_t *at;          /* device [n]: read by ar_hip_pages_write and ar_hip_attention_paged, filled in by
                              ar_hip_pages_grow */
     int32_t n;            /* chunks, 1 .. 2^20 */
-    int32_t rows;         /* rows of the call's row arrays, >= 0, at least start[n] */
+    int32_t rows;         /* rows of the call's row arrays, 0 .. 2^22, at least start[n] */
 } ar_chunks;
 
 /* Rotary positions with one to four axes (text; or time, height and width of images and video).  Frequency f of
@@ -74,7 +74,7 @@ typedef struct ar_rotary {
     int32_t section[4];
 } ar_rotary;
 
-/* Scratch bytes of ar_hip_pages_grow, _fork (n entries each), _compact and _copy (n entries) on these pages. */
+/* Scratch bytes of ar_hip_pages_grow and _fork (of n entries) and of _compact (n = 0) on these pages. */
 int ar_hip_pages_work(const ar_pages *pages, int n, size_t *bytes);
 
 /* Makes room for every chunk's rows at its sequence's end: at[i] = rows[seq[i]], which then grows by the chunk's
@@ -82,8 +82,9 @@ int ar_hip_pages_work(const ar_pages *pages, int n, size_t *bytes);
  * that is not full and that other sequences hold too is replaced by a copy of it; of several chunks on one such
  * page the last keeps it if no one else holds it.  A chunk that cannot be served, because the pool has no pages left
  * for it (then none that needs pages after it is served, either), its table row has no columns left, its sequence is
- * unknown or was named by an earlier chunk, leaves its sequence as it was and gets at[i] = -1.  *missing (device, or null) receives the number of pages that were wanted
- * beyond the free ones.  chunks->n at most 4096; needs rows and refs. */
+ * unknown or was named by an earlier chunk, leaves its sequence as it was and gets at[i] = -1.  *missing (device, or
+ * null) receives the number of pages that were wanted beyond the free ones.  chunks->n at most 4096; needs rows and
+ * refs. */
 int ar_hip_pages_grow(ar_hip_ctx *ctx, const ar_pages *pages, const ar_chunks *chunks, int32_t *missing, void *work,
                       size_t work_bytes);
 
@@ -126,9 +127,13 @@ int ar_hip_pages_write(ar_hip_ctx *ctx, const ar_pages *pages, int layer, const 
 /* Causal attention of every chunk's rows over their sequences' pages in one layer: the row at cache row p sees rows
  * 0 .. p (the chunk's own among them, written before), scores scaled by 1 / sqrt(head_dim), head h reads KV head
  * h / (heads / kv_heads).  q and out: [rows][heads * head_dim] of act_dtype (AR_DTYPE_F32 or AR_DTYPE_BF16), 16-byte
- * aligned.  Rows that see nothing become 0.  What a hidden row holds (infinities, NaN) does not reach the result.
- * Products and sums keep at least fp32's precision with fp32 activations; with bf16 activations the softmax weights
- * are rounded to 16 bits for the second product. */
+ * aligned; out may be q itself.  Rows that see nothing become 0.  What a hidden row holds (infinities, NaN) does not
+ * reach the result; infinities and NaN that a row sees make it infinite or NaN.
+ * Sums are in fp32.  With fp32 activations the products keep 22 bits or more: relative to each factor over 16-bit
+ * caches, to the largest value of its row of the cache over fp32 ones, and what a weight of less than 2^-30 of its
+ * row's largest loses is below 2^-30 of the value that it weighs.  With bf16 activations the softmax weights are
+ * rounded to 16 bits (the cache's type; fp16 for fp32 caches) for the second product.
+ * (chunks->rows * heads is at most 2^27, and no more than 2^23 tiles of 16 packed rows.) */
 int ar_hip_attention_paged_work(ar_hip_ctx *ctx, const ar_pages *pages, const ar_chunks *chunks, int heads,
                                 size_t *bytes);
 int ar_hip_attention_paged(ar_hip_ctx *ctx, const ar_pages *pages, int layer, const ar_chunks *chunks, const void *q,

@@ -10,6 +10,8 @@ fp16 2^-11):
       at most pi each for sin and cos, 4 u with their own error), 16 u of the head's largest value; storing adds r.
 Table calls and copies are exact.
 """
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -277,6 +279,194 @@ def test_attention_repeats_bit_for_bit(ctx):
     a = [_attend(ctx, pool, 0, [4999, 690], [1, 7], q, "f32", 8) for _ in range(4)]
     for b in a[1:]:
         np.testing.assert_array_equal(a[0], b)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("bf16", "f32"), ("bf16", "f16")])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [90, 3, 150]])
+def test_unknown_sequences_see_nothing(ctx, act, dtype, counts):
+    """Sequence numbers far past the table among proper ones, for one token each and for chunks."""
+    r = _rng(41)
+    pool = Pool(ctx, r, dtype, 1, 2, 64, 32, [300, 200])
+    q = r.standard_normal((sum(counts), 4, 64))
+    at = [40, 190, 30]
+    for seq in ([2 ** 31 - 1, 1, 0], [2, -2 ** 31, 1], [0, 1 << 29, 1], [2, 3, 4]):
+        got = _attend(ctx, pool, 0, at, counts, q, act, 4, seq=seq)
+        _check_attention(got, pool, 0, at, counts, q, act, 4, seq=seq)
+    pool.free()
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("at,counts", [([700, 3], [1, 1]), ([300], [160]), ([5, 90, 0], [70, 1, 40])])
+def test_rows_of_very_different_magnitudes(ctx, act, hd, at, counts):
+    """fp32 key and value rows from 1e-12 to 1e12, so that the largest value often has next to no weight and the
+    largest contribution changes along the keys.  Errors are relative to the contributions' largest dim."""
+    r = _rng(43)
+    pool = Pool(ctx, r, "f32", 1, 2, hd, 16, [a + c for a, c in zip(at, counts)])
+    shape = pool.v.shape[:4] + (1,)
+    pool.set("v", (pool.v * 10.0 ** r.uniform(-12, 12, shape)).astype(np.float32))
+    pool.set("k", (pool.k * 10.0 ** r.uniform(-12, 0.5, shape)).astype(np.float32))
+    q = 3 * r.standard_normal((sum(counts), 4, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    starts = _starts(counts)
+    pairs = [pool.seen(0, i) for i in range(len(counts))]
+    qv = ref.values(ref.to_bits(q, act))
+    want = ref.attention([qv[starts[i]:starts[i + 1]] for i in range(len(counts))], [p[0] for p in pairs],
+                         [p[1] for p in pairs], at, counts, 4)
+    half = HALF_STEP[act]
+    # (bf16 activations over fp32 rows: weights of 11 bits)
+    for i, (out, mag, big) in enumerate(want):
+        tol = ((64 * U * big + 32 * U + (2.0 ** -11 if act == "bf16" else 0)) * mag).max(-1, keepdims=True) + half * np.abs(out)
+        err = np.abs(got[starts[i]:starts[i + 1]] - out)
+        assert (err <= tol).all(), (i, (err / tol).max())
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("bf16", "f32"), ("bf16", "bf16"), ("bf16", "f16")])
+def test_a_first_tile_of_scores_of_minus_infinity(ctx, act, dtype):
+    """Visible keys whose scores are -inf have no weight, also where nothing else has been seen yet.  (bf16 queries: of
+    several planes some are 0 or of the other sign, and infinite keys make the row NaN.)"""
+    r = _rng(47)
+    at, counts = [200, 200], [1, 140]
+    pool = Pool(ctx, r, dtype, 1, 1, 64, 64, [201, 340])
+    bits = ref.to_bits(np.full(1, -np.inf), dtype)[0]
+    for i in range(2):
+        pool.k[0, pool.table[i, :2], :, :, 0] = bits
+    pool.set("k", pool.k)
+    q = r.standard_normal((sum(counts), 4, 64))
+    q[..., 0] = 1 + np.abs(q[..., 0])
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    rest = Pool.__new__(Pool)  # the same rows without the first two pages
+    rest.__dict__.update(pool.__dict__)
+    rest.table = pool.table.copy()
+    rest.table[:, :2] = -1
+    _check_attention(got, rest, 0, at, counts, q, act, 4)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("case", ["ones", "ones-starts", "mixed", "slots-few", "slots-mixed"])
+def test_attention_of_many_chunks(ctx, act, dtype, case):
+    """More chunks than a wavefront has lanes, and than one call cuts the keys of; empty ones among them."""
+    r = _rng(53)
+    n = {"ones": 150, "ones-starts": 150, "mixed": 150, "slots-few": 1100, "slots-mixed": 1100}[case]
+    counts = [1] * n
+    if case in ("ones-starts", "slots-few"):
+        counts = r.integers(0, 3, n).tolist()
+    if "mixed" in case:
+        counts = [int(r.integers(60, 150)) if i % (7 if n < 1000 else 9) == 3 else int(r.integers(0, 4)) for i in range(n)]
+        if case == "mixed":
+            counts[70] = 700
+    KV, G, hd = 2, 4, 64
+    seqs = 5
+    lengths = [900, 40, 333, 0, 128]
+    pool = Pool(ctx, r, dtype, 1, KV, hd, 32, lengths)
+    seq = r.integers(0, seqs, n).tolist()
+    at = [max(0, int(r.integers(0, max(1, lengths[s] - c + 1)))) for s, c in zip(seq, counts)]
+    if case == "ones":
+        seq = None
+        pool.free()
+        lengths = r.integers(0, 300, n).tolist()
+        pool = Pool(ctx, r, dtype, 1, KV, hd, 32, lengths)
+        at = [x - 1 for x in lengths]
+    total = sum(counts)
+    q = r.standard_normal((total, KV * G, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, act, KV * G, seq=seq, one_each=case == "ones", extra=0 if case == "ones" else 2)
+    pick = [i for i in range(n) if i < 3 or i > n - 4 or i % 13 == 3 or i == 70]  # (the 64-bit reference is slow)
+    starts = _starts(counts)
+    rows = np.concatenate([np.arange(starts[i], starts[i + 1]) for i in pick])
+    some = [counts[i] for i in pick]
+    _check_attention(got[rows], pool, 0, [at[i] for i in pick], some, q[rows], act, KV * G,
+                     seq=[i if seq is None else seq[i] for i in pick])
+    assert np.isfinite(got).all()
+    pool.free()
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(96, 96, 64), (40, 40, 128), (300, 3, 64)])
+@pytest.mark.parametrize("counts", [[1, 1], [33, 1]])
+def test_attention_of_many_heads(ctx, heads, kv, hd, counts):
+    r = _rng(59)
+    at = [150, 77]
+    pool = Pool(ctx, r, "bf16", 1, kv, hd, 16, [a + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), heads, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, "bf16", heads)
+    _check_attention(got, pool, 0, at, counts, q, "bf16", heads)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("at,counts", [([3000, 20], [1, 1]), ([600], [150]), ([10, 5, 900], [90, 1, 30])])
+def test_attention_in_place(ctx, act, dtype, at, counts):
+    """The output over the queries, whether the keys are cut or not."""
+    r = _rng(61)
+    pool = Pool(ctx, r, dtype, 1, 2, 64, 64, [a + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), 8, 64))
+    apart = _attend(ctx, pool, 0, at, counts, q, act, 8)
+    host = ref.to_bits(q, act)
+    qd, ad, sd = ctx.to_device(host), _i32(ctx, at), _i32(ctx, _starts(counts))
+    pool.cache.attention(0, pg.Chunks(len(counts), len(q), at=ad, start=sd), qd, qd, 8, CODE[act])
+    ctx.synchronize()
+    np.testing.assert_array_equal(ref.values(qd.download(host.dtype, host.size).reshape(host.shape)), apart)
+    for b in (qd, ad, sd):
+        b.free()
+    pool.free()
+
+
+def test_attention_refuses_on_a_context(ctx):
+    """Work space that is missing, too small or not aligned, and more rows than a launch has blocks for."""
+    r = _rng(67)
+    pool = Pool(ctx, r, "f16", 1, 2, 64, 16, [3000])
+    q, o, at = (ctx.allocate(8 * 4 * 64 * 4) for _ in range(3))
+    at.upload(np.zeros(8, np.int32))
+    ch = pg.Chunks(1, 1, at=at)
+    need = ctypes.c_size_t()
+    L = hw.lib()
+    hw.check(L.ar_hip_attention_paged_work(ctx.handle, pool.cache.ref, ch.ref, 4, ctypes.byref(need)))
+    w = ctx.allocate(need.value + 16)
+
+    def call(work, nbytes, chunks=ch, heads=4):
+        rc = L.ar_hip_attention_paged(ctx.handle, pool.cache.ref, 0, chunks.ref, q.ptr, 0, heads, o.ptr, work, nbytes)
+        return rc, L.ar_hip_last_error().decode()
+
+    for work, nbytes, word in ((None, need.value, "needed"), (w.ptr, need.value - 1, "needed"), (w.ptr + 8, need.value, "aligned")):
+        rc, text = call(work, nbytes)
+        assert rc == hw.AR_HIP_ERR_INVALID and word in text, text
+    assert call(w.ptr, need.value)[0] == 0
+    assert call(w.ptr, 0, pg.Chunks(1, 0, at=at, start=at))[0] == 0  # no rows: nothing to do
+    many = pg.Chunks(1, 1 << 22, at=at, start=at)
+    rc = L.ar_hip_attention_paged_work(ctx.handle, pool.cache.ref, many.ref, 1 << 10, ctypes.byref(need))
+    assert rc == hw.AR_HIP_ERR_INVALID and "too many" in L.ar_hip_last_error().decode()
+    ctx.synchronize()
+    for b in (q, o, at, w):
+        b.free()
+    pool.free()
+
+
+def test_two_contexts_at_once(ctx):
+    """One pool read on two streams at the same time, each with its own work space."""
+    r = _rng(71)
+    pool = Pool(ctx, r, "bf16", 1, 2, 128, 64, [4000, 900, 2500])
+    at, counts = [3990, 890, 2490], [10, 1, 1]
+    q = r.standard_normal((12, 8, 128))
+    want = _attend(ctx, pool, 0, at, counts, q, "bf16", 8)
+    host = ref.to_bits(q, "bf16")
+    with hw.HipContext(0) as other:
+        sides = []
+        for c in (ctx, other):
+            cache = pg.PagedCache(c, 1, len(pool.refs), 2, 128, 3, pool.table.shape[1], page_rows=64, dtype=CODE["bf16"],
+                                  **pool.buf)
+            sides.append((c, cache, c.to_device(host), c.allocate(host.nbytes), _i32(c, at), _i32(c, _starts(counts))))
+        for _ in range(20):
+            for c, cache, qd, od, ad, sd in sides:
+                cache.attention(0, pg.Chunks(3, 12, at=ad, start=sd), qd, od, 8, CODE["bf16"])
+        for c, cache, *bufs in sides:
+            c.synchronize()
+            np.testing.assert_array_equal(ref.values(bufs[1].download(host.dtype, host.size).reshape(host.shape)), want)
+        for c, cache, *bufs in sides:
+            cache.close()
+            for b in bufs:
+                b.free()
     pool.free()
 
 

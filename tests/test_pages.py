@@ -100,16 +100,19 @@ def test_null_structures_and_context_are_refused():
     _refused(_attend(p, None), "null")
     _refused(_write(p, c, None), "rotary axes")
     # nothing else wrong: the context is
-    for rc in (_grow(p, c), _attend(p, c), _write(p, c, _rotary()), L.ar_hip_pages_trim(None, ctypes.byref(p), None, None, 3),
-               L.ar_hip_pages_fork(None, ctypes.byref(p), A, A, 2, A, 1 << 20),
-               L.ar_hip_pages_compact(None, ctypes.byref(p), None, A, 1 << 20),
-               L.ar_hip_pages_copy(None, ctypes.byref(p), ctypes.byref(_pages(k=A * 3, v=A * 4)), A, A, 1),
-               L.ar_hip_attention_paged_work(None, ctypes.byref(p), ctypes.byref(c), 4, ctypes.byref(b))):
-        _refused(rc, "ctx is null")
+    other = _pages(k=1 << 40, v=1 << 41)
+    for call in (lambda: _grow(p, c), lambda: _attend(p, c), lambda: _write(p, c, _rotary()),
+                 lambda: L.ar_hip_pages_trim(None, ctypes.byref(p), None, None, 3),
+                 lambda: L.ar_hip_pages_fork(None, ctypes.byref(p), A, A, 2, A, 1 << 20),
+                 lambda: L.ar_hip_pages_compact(None, ctypes.byref(p), None, A, 1 << 20),
+                 lambda: L.ar_hip_pages_copy(None, ctypes.byref(p), ctypes.byref(other), A, A, 1),
+                 lambda: L.ar_hip_attention_paged_work(None, ctypes.byref(p), ctypes.byref(c), 4, ctypes.byref(b))):
+        _refused(call(), "ctx is null")
 
 
 @pytest.mark.parametrize("over,word", [(dict(at=None), "cache rows"), (dict(n=0), "chunks"), (dict(n=-1), "chunks"),
                                        (dict(n=(1 << 20) + 1), "chunks"), (dict(rows=-1), "negative"),
+                                       (dict(rows=(1 << 22) + 1), "2^22"),
                                        (dict(start=None, n=3, rows=2), "one row"), (dict(n=4), "sequences")])
 def test_bad_chunks_are_refused(over, word):
     p, c = _pages(), _chunks(**over)
@@ -155,6 +158,13 @@ def test_copy_refuses_pools_of_another_shape(over):
 
 def test_copy_refuses_pools_that_share_part_of_their_memory():
     L, p = hw.lib(), _pages()
+    # (a pool array of _pages: 2 layers of 8 pages, 2 heads, 16 rows, 64 dims of fp32)
+    size = p.layers * p.pages * p.kv_heads * p.page_rows * p.head_dim * 4
+    big = _pages(k=1 << 40, v=(1 << 40) + 100 * size)
+    for over in (dict(k=big.k + size - 16, v=big.v + 8 * size), dict(k=big.k - size + 16, v=big.v + 8 * size),
+                 dict(k=big.v + 16, v=big.v + 8 * size), dict(k=big.k + 8 * size, v=big.v + size - 16),
+                 dict(k=big.k - 2 * size + 16, v=big.v + 8 * size, pages=2 * big.pages)):
+        _refused(L.ar_hip_pages_copy(None, ctypes.byref(big), ctypes.byref(_pages(**over)), A, A, 1), "share")
     for over, word in ((dict(v=3 * A), "share"), (dict(k=2 * A, v=A), "share"), (dict(pages=9), "two page counts")):
         _refused(L.ar_hip_pages_copy(None, ctypes.byref(p), ctypes.byref(_pages(**over)), A, A, 1), word)
 
@@ -193,3 +203,43 @@ def test_binding_refuses_before_the_library():
         pg.Rotary(1e6, None, [8, 8, 8, 4, 4])
     with pytest.raises(ValueError):
         pg.PagedCache(None, 1, 1, 1, 64, 1, 1, dtype=hw.DTYPE_F64)
+
+
+def test_calls_after_close_are_refused():
+    """A closed cache hands no freed pointer on."""
+    class Buf:
+        def __init__(self, nbytes=0):
+            self.ptr, self.nbytes, self.freed = A, nbytes, False
+
+        def upload(self, a):
+            pass
+
+        def free(self):
+            self.freed = True
+
+    class Ctx:
+        handle = None
+
+        def __init__(self):
+            self.made = []
+
+        def allocate(self, nbytes):
+            self.made.append(Buf(nbytes))
+            return self.made[-1]
+
+    ctx, given = Ctx(), Buf()
+    cache = pg.PagedCache(ctx, 1, 4, 1, 64, 2, 2, v=given)
+    cache._scratch(100)
+    first = cache._work[-1]
+    cache._scratch(90)
+    assert cache._work == [first]
+    cache._scratch(101)  # queued calls may use the first: it stays
+    assert not first.freed and cache._work[-1].nbytes >= 200
+    at = Buf()
+    ch = pg.Chunks(1, 1, at=at)
+    cache.close()
+    assert all(b.freed for b in ctx.made) and not given.freed
+    for call in (lambda: cache.grow(ch), lambda: cache.trim(None, None, 1), lambda: cache.attention(0, ch, at, at, 1),
+                 lambda: cache.compact(), lambda: cache.copy(cache, at, at, 1)):
+        with pytest.raises(Exception, match="no keys"):
+            call()
