@@ -100,6 +100,15 @@ __device__ __forceinline__ void split2(float x, float y, unsigned* out) {
     if constexpr (N > 2) out[2] = E::pack(x - E::low(out[1]), y - E::high(out[1]));
 }
 
+// Two fp16 planes of a value times a power of two, each in one mixed-precision multiply-add per value.
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split2_scaled(float x, float y, float scale, unsigned* out) {
+    const halfx2 a = {(_Float16)fmaf(x, scale, 0.f), (_Float16)fmaf(y, scale, 0.f)};
+    const halfx2 b = {(_Float16)fmaf(x, scale, -(float)a.x), (_Float16)fmaf(y, scale, -(float)a.y)};
+    out[0] = __builtin_bit_cast(unsigned, a);
+    out[1] = __builtin_bit_cast(unsigned, b);
+}
+
 // fp32 products: a (bits) x b, 16 x 16 x 4
 __device__ __forceinline__ floatx4 mac4f(unsigned a, float b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), b, c, 0, 0, 0);
@@ -110,14 +119,15 @@ __device__ __forceinline__ floatx4 mac4(unsigned a, unsigned b, floatx4 c) { ret
 // at most 2^100, also for a row of zeros.
 __device__ __forceinline__ int fp16_shift(float top) { return min(141 - (int)(__float_as_uint(top) >> 23), 100); }
 
-// maximum over the LANES (8 or 16) lanes that hold a row
+// maximum over the LANES (8 or 16) lanes that hold a row; of values >= 0, as their bits (which need no canonical form)
 template <int LANES>
-__device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, dpp_mov<0xB1, 0xF>(v));   // quad_perm 1,0,3,2
-    v = fmaxf(v, dpp_mov<0x4E, 0xF>(v));   // quad_perm 2,3,0,1
-    v = fmaxf(v, dpp_mov<0x141, 0xF>(v));  // row_half_mirror
-    if (LANES == 16) v = fmaxf(v, dpp_mov<0x140, 0xF>(v));  // row_mirror
-    return v;
+__device__ __forceinline__ float row_max(float value) {
+    unsigned v = __float_as_uint(value);
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));   // quad_perm 1,0,3,2
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));   // quad_perm 2,3,0,1
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));  // row_half_mirror
+    if (LANES == 16) v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));  // row_mirror
+    return __uint_as_float(v);
 }
 
 // A piece of values (of fp32 or 16-bit ones) with zeros for infinities and NaN, which a hidden key's weight of 0 would
@@ -497,23 +507,23 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                     v[i] = __uint_as_float(st[2 * u + i / 4][i % 4]);
                     top = fmaxf(top, fabsf(v[i]));
                 }
-                float sum = 0.f;  // (NaN where there is one)
-#pragma unroll
-                for (int i = 0; i < 8; i++) sum = fmaf(v[i], 0.f, sum);
                 top = row_max<C::CPR>(top);
-                const bool special = __ballot(!(top < INFINITY) || sum != 0.f);
-                if (__builtin_expect(special, 0)) {  // the largest finite value of the row
-                    top = 0.f;
+                int e = fp16_shift(top);
+                float scale = __uint_as_float((unsigned)(e + 127) << 23);
+                unsigned pl[4][NK];
+                halfx2 zero = {0, 0};  // (NaN where an infinity or NaN is)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    split2_scaled(v[2 * i], v[2 * i + 1], scale, pl[i]);
+                    zero = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, pl[i][0]), halfx2{0, 0}, zero);
+                }
+                if (__builtin_expect(__ballot(__builtin_bit_cast(unsigned, zero) != 0) != 0, 0)) {
+                    top = 0.f;  // the largest finite value of the row
 #pragma unroll
                     for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
                     top = row_max<C::CPR>(top);
-                }
-                const int e = fp16_shift(top);
-                const float scale = __uint_as_float((unsigned)(e + 127) << 23);
-                unsigned pl[4][NK];
-#pragma unroll
-                for (int i = 0; i < 4; i++) split2<true, NK, false>(v[2 * i] * scale, v[2 * i + 1] * scale, pl[i]);
-                if (__builtin_expect(special, 0)) {
+                    e = fp16_shift(top);
+                    scale = __uint_as_float((unsigned)(e + 127) << 23);
 #pragma unroll
                     for (int i = 0; i < 4; i++) split2<true, NK, true>(v[2 * i] * scale, v[2 * i + 1] * scale, pl[i]);
                 }
@@ -662,13 +672,18 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
             }
             return (sum[0] + sum[1]) + (sum[2] + sum[3]);
         };
-        auto products = [&](int kt) __attribute__((always_inline)) {
+        auto products = [&](int kt, float scale) __attribute__((always_inline)) {  // (scale: of fp32 caches)
 #pragma unroll
             for (int k2 = 0; k2 < 2; k2++) {
                 if (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // one step's planes at a time: registers
                 unsigned u[4][NQ];
 #pragma unroll
-                for (int i = 0; i < 4; i++) split2<C::F16, NQ, false>(s[kt][8 * k2 + 2 * i], s[kt][8 * k2 + 2 * i + 1], u[i]);
+                for (int i = 0; i < 4; i++) {
+                    const float x = s[kt][8 * k2 + 2 * i], y = s[kt][8 * k2 + 2 * i + 1];
+                    if constexpr (!C::KF) split2<C::F16, NQ, false>(x, y, u[i]);
+                    else if constexpr (NQ == 1) split2<true, 1, false>(x * scale, y * scale, u[i]);
+                    else split2_scaled(x, y, scale, u[i]);
+                }
                 u32x4 pf[NQ];
 #pragma unroll
                 for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
@@ -703,11 +718,11 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                 if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
                 if (!__ballot(!(fmaf(mx, c, -m) <= kSlack))) {  // (no key seen yet: NaN or infinity)
                     if (NQ > 1) __builtin_amdgcn_s_setprio(1);
-                    products(0);
+                    products(0, 1.f);
                     if (NQ > 1) __builtin_amdgcn_s_setprio(0);
                     if constexpr (KT32 > 1) {
                         sum += weights(1, mu);
-                        products(1);
+                        products(1, 1.f);
                     }
                     l += sum;
                     continue;
@@ -744,7 +759,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         float mx = largest(0);
         if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
         mx = max_xor32(mx) * c;
-        if (__ballot(mx > m)) {
+        if (__ballot(mx - m > kSlack)) {  // (no key seen before: infinity; none yet: NaN)
             const float mn = fmaxf(m, mx);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= alpha;
@@ -759,6 +774,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         const float mu = m == -INFINITY ? 0.f : m - C::BIAS;
 #pragma unroll
         for (int kt = 0; kt < KT32; kt++) l += weights(kt, mu);
+        float scale = 1.f;
         if constexpr (C::KF) {
             // weights take over the values' powers of two, and a power of the row's that brings the largest so far
             // into [2^3, 2^15]: bits are lost relative to the largest contribution, not to the largest value
@@ -780,14 +796,10 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                     for (int r = 0; r < 16; r++) o[j][r] = ldexpf(o[j][r], to - ve);
                 ve = to;
             }
-            const float scale = __uint_as_float((unsigned)(ve + 127) << 23);
-#pragma unroll
-            for (int kt = 0; kt < KT32; kt++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[kt][r] *= scale;
+            scale = __uint_as_float((unsigned)(ve + 127) << 23);
         }
 #pragma unroll
-        for (int kt = 0; kt < KT32; kt++) products(kt);
+        for (int kt = 0; kt < KT32; kt++) products(kt, scale);
         if (__builtin_expect(bad, 0)) {
             // the values that were left out: their weights are positive, so that each is its own contribution
 #pragma unroll 1
