@@ -494,46 +494,78 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
             }
         }
     };
-    auto stage_store = [&](const Staged& st, int odd, int values) __attribute__((always_inline)) {
+    auto staged_at = [&](int u, int odd, int values) __attribute__((always_inline)) {
+        const int piece = u * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
+        const int x = values ? value_swizzle(key) : HD == 128 ? key & 15 : (key >> 1) & 7;
+        return lds + (2 * odd + values) * C::TILE + key * (HD * 2) + ((col ^ x) * 16);
+    };
+    // Staged rows into LDS.  fp32 ones become two fp16 planes and a power of two, in kSteps steps a piece, each short
+    // enough to run under one matrix instruction, and free of branches: `special` becomes nonzero if one holds an
+    // infinity or NaN (then stage_special does the work again).
+    constexpr int kSteps = 6;
+    float p_scale = 0.f;
+    unsigned p_plane[4][2], special = 0;
+    halfx2 p_zero = {0, 0};
+    auto stage_step = [&](const Staged& st, int u, int part, int odd, int values) __attribute__((always_inline)) {
+        auto value = [&](int i) __attribute__((always_inline)) { return __uint_as_float(st[2 * u + i / 4][i % 4]); };
+        if (part == 0) {
+            p_scale = fabsf(value(0));
+#pragma unroll
+            for (int i = 1; i < 8; i++) p_scale = fmaxf(p_scale, fabsf(value(i)));
+            p_zero = halfx2{0, 0};
+        } else if (part == 1) {
+            const int e = fp16_shift(row_max<C::CPR>(p_scale));
+            p_scale = __uint_as_float((unsigned)(e + 127) << 23);
+            s_exp[odd][values][(u * kThreads + tid) / C::CPR] = -e;  // (by all of the row's lanes)
+        } else {
+            const int i = part - 2;
+            split2_scaled(value(2 * i), value(2 * i + 1), p_scale, p_plane[i]);
+            p_zero = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, p_plane[i][0]), halfx2{0, 0}, p_zero);  // (NaN)
+            if (i == 3) {
+                special |= __builtin_bit_cast(unsigned, p_zero);
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+                    *reinterpret_cast<u32x4*>(staged_at(u, odd, values) + n * C::PLANE) =
+                        quad(p_plane[0][n], p_plane[1][n], p_plane[2][n], p_plane[3][n]);
+            }
+        }
+    };
+    // step n of a tile's: its keys' pieces, then its values'
+    auto stage_nth = [&](int n, int odd) __attribute__((always_inline)) {
+        const int piece = n / kSteps;
+        if (piece < C::UNITS) stage_step(sk, piece, n % kSteps, odd, 0);
+        else stage_step(sv, piece - C::UNITS, n % kSteps, odd, 1);
+    };
+    auto stage_store = [&](int odd) __attribute__((always_inline)) {
+        if constexpr (C::KF) {
+#pragma unroll
+            for (int n = 0; n < 2 * C::UNITS * kSteps; n++) stage_nth(n, odd);
+        } else {
+#pragma unroll
+            for (int u = 0; u < C::UNITS; u++) *reinterpret_cast<u32x4*>(staged_at(u, odd, 0)) = sk[u];
+#pragma unroll
+            for (int u = 0; u < C::UNITS; u++) *reinterpret_cast<u32x4*>(staged_at(u, odd, 1)) = sv[u];
+        }
+    };
+    auto stage_special = [&](const Staged& st, int odd, int values) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < C::UNITS; u++) {
-            const int piece = u * kThreads + tid, key = piece / C::CPR, col = piece % C::CPR;
-            const int x = values ? value_swizzle(key) : HD == 128 ? key & 15 : (key >> 1) & 7;
-            char* dst = lds + (2 * odd + values) * C::TILE + key * (HD * 2) + ((col ^ x) * 16);
-            if constexpr (C::KF) {
-                float v[8], top = 0.f;
+            char* dst = staged_at(u, odd, values);
+            float v[8], top = 0.f;  // the largest finite value of the row
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    v[i] = __uint_as_float(st[2 * u + i / 4][i % 4]);
-                    top = fmaxf(top, fabsf(v[i]));
-                }
-                top = row_max<C::CPR>(top);
-                int e = fp16_shift(top);
-                float scale = __uint_as_float((unsigned)(e + 127) << 23);
-                unsigned pl[4][NK];
-                halfx2 zero = {0, 0};  // (NaN where an infinity or NaN is)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    split2_scaled(v[2 * i], v[2 * i + 1], scale, pl[i]);
-                    zero = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, pl[i][0]), halfx2{0, 0}, zero);
-                }
-                if (__builtin_expect(__ballot(__builtin_bit_cast(unsigned, zero) != 0) != 0, 0)) {
-                    top = 0.f;  // the largest finite value of the row
-#pragma unroll
-                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
-                    top = row_max<C::CPR>(top);
-                    e = fp16_shift(top);
-                    scale = __uint_as_float((unsigned)(e + 127) << 23);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) split2<true, NK, true>(v[2 * i] * scale, v[2 * i + 1] * scale, pl[i]);
-                }
-#pragma unroll
-                for (int n = 0; n < NK; n++)
-                    *reinterpret_cast<u32x4*>(dst + n * C::PLANE) = quad(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
-                if (col == 0) s_exp[odd][values][key] = -e;
-            } else {
-                *reinterpret_cast<u32x4*>(dst) = st[u];
+            for (int i = 0; i < 8; i++) {
+                v[i] = __uint_as_float(st[2 * u + i / 4][i % 4]);
+                top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
             }
+            const int e = fp16_shift(row_max<C::CPR>(top));
+            const float scale = __uint_as_float((unsigned)(e + 127) << 23);
+            unsigned pl[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split2<true, 2, true>(v[2 * i] * scale, v[2 * i + 1] * scale, pl[i]);
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+                *reinterpret_cast<u32x4*>(dst + n * C::PLANE) = quad(pl[0][n], pl[1][n], pl[2][n], pl[3][n]);
+            s_exp[odd][values][(u * kThreads + tid) / C::CPR] = -e;  // (by all of the row's lanes)
         }
     };
     // Zeros this thread's pieces of values that are not there, infinities and NaN, in LDS; whether there were any of
@@ -561,11 +593,16 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         if (pg3 < 0 && (3 << p.shift) < BK) miss |= page_keys << ((3 << p.shift) & 63);
         return miss;
     };
-    // The staged tile into LDS; where some row of the block does not see all of it, its values are cleaned.
-    auto stage_tile = [&](int tile, unsigned long long miss) __attribute__((always_inline)) {
+    // What the staged tile needs besides; where some row of the block does not see all of it, its values are cleaned.
+    auto stage_rest = [&](int tile, unsigned long long miss) __attribute__((always_inline)) {
         const int odd = tile & 1;
-        stage_store(sk, odd, 0);
-        stage_store(sv, odd, 1);
+        if constexpr (C::KF) {
+            if (__builtin_expect(__ballot(special != 0) != 0, 0)) {
+                stage_special(sk, odd, 0);
+                stage_special(sv, odd, 1);
+                special = 0;
+            }
+        }
         if (tile < t1 && (miss != 0 || tile * BK + BK - 1 > blim0) && clean(odd, tile * BK, miss)) s_bad[odd] = tile;
     };
 
@@ -618,7 +655,8 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
     unsigned long long miss_next = 0;
     if (t0 < t1) {
         load_pages(t0 + 1);
-        stage_tile(t0, miss);
+        stage_store(t0 & 1);
+        stage_rest(t0, miss);
         miss_next = missing();
         stage_load(sk, t0 + 1, p.kp, pg0, pg1, pg2, pg3);
         stage_load(sv, t0 + 1, p.vp, pg0, pg1, pg2, pg3);
@@ -632,14 +670,6 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         const int k0 = tile * BK, odd = tile & 1;
         lds_barrier();
         const bool bad = s_bad[odd] == tile;
-        stage_tile(tile + 1, miss_next);
-        stage_load(sk, tile + 2, p.kp, pg0, pg1, pg2, pg3);
-        stage_load(sv, tile + 2, p.vp, pg0, pg1, pg2, pg3);
-        const unsigned long long miss_here = miss;
-        miss = miss_next;
-        miss_next = missing();
-        load_pages(tile + 3);
-
         const char* const kbuf = lds + 2 * odd * C::TILE;
         const char* const vbuf = kbuf + C::TILE;
         floatx16 s[KT32];
@@ -656,6 +686,44 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                         if (i + j < C::DEPTH) s[kt] = E::mac(kf, qf[i][ks], s[kt]);
                 }
         };
+        if constexpr (C::KF) {
+            // the next tile's planes are made under this one's matrix instructions
+            constexpr int kSteps0 = 2 * C::UNITS * kSteps, kMacs = KS * (NQ == 1 ? 2 : 3);
+            u32x4 kf[2][NK];
+            auto key_load = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < NK; j++) kf[ks & 1][j] = *reinterpret_cast<const u32x4*>(kbuf + j * C::PLANE + (kaddr ^ (ks * 32)));
+            };
+            key_load(0);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[0][r] = 0.f;
+            int n = 0;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if (ks + 1 < KS) key_load(ks + 1);
+#pragma unroll
+                for (int j = 0; j < NK; j++)
+#pragma unroll
+                    for (int i = 0; i < NQ; i++)
+                        if (i + j < C::DEPTH) {
+                            s[0] = E::mac(kf[ks & 1][j], qf[i][ks], s[0]);
+#pragma unroll
+                            for (int x = n * kSteps0 / kMacs; x < (n + 1) * kSteps0 / kMacs; x++) stage_nth(x, 1 - odd);
+                            n++;
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+            }
+        } else {
+            stage_store(1 - odd);
+        }
+        stage_rest(tile + 1, miss_next);
+        stage_load(sk, tile + 2, p.kp, pg0, pg1, pg2, pg3);
+        stage_load(sv, tile + 2, p.vp, pg0, pg1, pg2, pg3);
+        const unsigned long long miss_here = miss;
+        miss = miss_next;
+        miss_next = missing();
+        load_pages(tile + 3);
+
         auto largest = [&](int kt) __attribute__((always_inline)) {
             float mx = s[kt][0];
 #pragma unroll
@@ -729,9 +797,10 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
                 }
             }
         }
+        if constexpr (!C::KF) {
 #pragma unroll
-        for (int kt = 0; kt < KT32; kt++) scores(kt);
-        if constexpr (C::KF) {
+            for (int kt = 0; kt < KT32; kt++) scores(kt);
+        } else {
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
 #pragma unroll
