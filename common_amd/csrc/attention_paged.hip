@@ -31,7 +31,7 @@ __device__ __forceinline__ u32x4 quad(unsigned a, unsigned b, unsigned c, unsign
 // One kernel's share of a call.
 struct PartArgs {
     int tiles, tasks;     // at most
-    int target;           // how many tasks to cut the keys for (0: a tile is a task)
+    int target, blocks;   // how many tasks to cut the keys for (0: a tile is a task), and how many they may become
     float* part;          // [tasks][kv_heads][tile rows][hd] unnormalised outputs of splits, and (m, l) of each
     float2* part_ml;
 };
@@ -195,6 +195,11 @@ struct Shape {
 template <int ROWS>
 constexpr int kUnit = ROWS == 16 ? 128 : 64;  // a round of the few-row kernel's wavefronts; the tile kernel's largest key tile
 
+// Units of a split, at least.  (One token over 4,096 rows in splits of one unit: 17.0 us, of two 14.1; tiles over few keys
+// want all the blocks they can get: 509 tokens over 609 rows 33.5 us, with two units 36.7.)
+template <int ROWS>
+constexpr float kLeast = ROWS == 16 ? 2.f : 1.f;
+
 struct Task {
     int seq, first, count;  // chunk
     int at;                 // cache row of its first token
@@ -292,7 +297,17 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         }
         keys = __int_as_float(lane_value(__float_as_int(wave_sum_lane63(keys)), 63));
         // (a little more than the even share, for the sum's roundings)
-        const float share = fmaxf(1.f, ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)));
+        float share = fmaxf(kLeast<ROWS>, ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)));
+        // That many units in a split are surely few enough tasks, with one more a tile.  Few rows, where the lanes hold
+        // the units of all tiles: the fewest units whose tasks are all resident at once (16 sequences of 8,192 rows: 78 us
+        // instead of 82, 40 of 2,000: 59 instead of 68).
+        if (ROWS == 16 && p.n <= 64 && __ballot(n > 1) == 0) {
+            const float most = (float)min(p.few.blocks, p.few.tasks), u = (float)c.units, top = share;
+            for (share = fmaxf(kLeast<ROWS>, ceilf(keys / (most * kUnit<ROWS>)) - 1.f); share < top; share += 1.f) {
+                const float tasks = n == 0 ? 0.f : fmaxf(1.f, ceilf(u / share));
+                if (__int_as_float(lane_value(__float_as_int(wave_sum_lane63(tasks)), 63)) <= most) break;
+            }
+        }
         const double inv = 1. / ((double)share * kUnit<ROWS>);
         const int per = (int)fminf(share, 1 << 24);  // (no chunk has more units)
         int tasks = 0, tiles = 0;  // before this round's chunks
@@ -1308,10 +1323,10 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
 // ---- host side ----------------------------------------------------------------------------------------------
 
 // A kernel's share of a call: its tiles at most, and how many tasks to cut their keys into (0: none; one more per tile
-// for what rounding makes of it).
+// for its last split, and one for what rounding makes of where its tasks begin).
 struct Part {
-    int tiles = 0, target = 0;
-    int tasks() const { return target ? target + tiles + 1 : tiles; }
+    int tiles = 0, target = 0, blocks = 0;  // (blocks: resident at once)
+    int tasks() const { return target ? std::max(target + tiles + 1, blocks) : tiles; }
     size_t bytes(const ar_pages* p, int rows) const {
         return target ? (size_t)tasks() * p->kv_heads * rows * ((size_t)p->head_dim * 4 + 8) : 0;
     }
@@ -1329,14 +1344,14 @@ constexpr int kFewRows = 16, kMaxSplitChunks = 1024;
 
 // Tasks to cut the keys for: `per_cu` blocks a CU over all KV heads, the number that is resident at once, unless the tiles
 // alone are as many (1,024 tokens of three sequences, 537 tiles for 512 blocks: whole tiles 609 us, cut ones 632).
-int target_of(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu, int unit) {
-    if (tiles * p->kv_heads >= (long long)per_cu * ctx->num_cus || n > kMaxSplitChunks) return 0;
-    if ((long long)p->max_pages * p->page_rows <= unit) return 0;  // (one split of any sequence)
+void cut_keys(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu, int unit, Part* out) {
+    const long long blocks = (long long)per_cu * ctx->num_cus / p->kv_heads, cap = (long long)p->max_pages * p->page_rows;
+    if (tiles >= blocks || n > kMaxSplitChunks) return;
+    if (cap <= unit) return;  // (one split of any sequence)
     // (a tile's last split is a task of its own, so that there may be `tiles` more; and no more than units)
-    const long long cap = (long long)p->max_pages * p->page_rows;
-    const long long blocks = (long long)per_cu * ctx->num_cus / p->kv_heads - tiles;
-    const long long want = std::min(blocks, std::max<long long>(tiles, n) * ((cap + unit - 1) / unit));
-    return (int)std::max(1LL, want);
+    const long long want = std::min(blocks - tiles, std::max<long long>(tiles, n) * ((cap + unit - 1) / unit));
+    out->target = (int)std::max(1LL, want);
+    out->blocks = (int)blocks;
 }
 
 int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int heads, Plan* out) {
@@ -1349,13 +1364,13 @@ int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int he
     if (!c->start || packed <= 32LL * c->n) {
         a.few_rows = 0x7fffffff;
         a.few.tiles = (int)(c->start ? packed / 16 + c->n : c->n * ((group + 15) / 16));
-        a.few.target = target_of(ctx, p, std::max<long long>(c->n, packed / 16), c->n, few_cu, kUnit<16>);
+        cut_keys(ctx, p, std::max<long long>(c->n, packed / 16), c->n, few_cu, kUnit<16>, &a.few);
     } else {
         a.tile.tiles = (int)(packed / 128 + c->n);
-        a.tile.target = target_of(ctx, p, packed / 128, c->n, tile_cu, kUnit<128>);
+        cut_keys(ctx, p, packed / 128, c->n, tile_cu, kUnit<128>, &a.tile);
         if (c->n > 1) {
             a.few_rows = kFewRows;
-            a.few.target = target_of(ctx, p, 0, c->n, few_cu, kUnit<16>);
+            cut_keys(ctx, p, 0, c->n, few_cu, kUnit<16>, &a.few);
             a.few.tiles = (int)(a.few.target ? std::min(packed / 16 + c->n, kFewRows / 16LL * c->n) : packed / 16 + c->n);
         }
     }
@@ -1368,7 +1383,7 @@ size_t plan_bytes(const ar_pages* p, const Plan& a) { return std::max<size_t>(16
 template <int HD, typename QT, typename KT>
 int launch_plan(const ar_pages* pages, const Plan& a, PagedParams p, char* work, hipStream_t st) {
     auto part = [&](const Part& x, int rows, char* at) {
-        return PartArgs{x.tiles, x.tasks(), x.target, (float*)at, (float2*)(at + (size_t)x.tasks() * p.kv_heads * rows * HD * 4)};
+        return PartArgs{x.tiles, x.tasks(), x.target, x.blocks, (float*)at, (float2*)(at + (size_t)x.tasks() * p.kv_heads * rows * HD * 4)};
     };
     p.few = part(a.few, 16, work);
     p.tile = part(a.tile, 128, work + a.few.bytes(pages, 16));
