@@ -3,15 +3,27 @@
 //   out_r = sum_j w_rj v_j / sum_j w_rj,   w_rj = exp(q_r k_j / sqrt(hd) - m_r),   j <= position of r, j on a page
 //
 // in one pass over the keys with a running maximum m and sum l.  The rows of a chunk's query heads that share a KV head
-// are packed (row t * G + g: token t, head g of the group), so that a tile of 32 rows uses every key G times more often,
-// and both products run on the matrix units, transposed, so that a lane owns one row and the weights feed the second
+// are packed (row t * G + g: token t, head g of the group), so that a tile of rows uses every key G times more often.
+// Two kernels share the work by a chunk's packed rows: the tile kernel (many rows, bound by the matrix units and by the
+// softmax's vector instructions) and the few-row kernel (decode steps, bound by HBM); where the keys are cut among
+// blocks, a merge kernel adds the parts up in a fixed order.
+//
+// Both products run on the matrix units, transposed, so that a lane owns one row and the weights feed the second
 // product from the registers the first one left them in:
 //   S^T (32 keys x 32 rows) = K Q^T    A: lane l has key l % 32, dims 16 s + 8 (l / 32) .. + 7 of step s
 //   O^T (hd x 32 rows)     += V^T P^T  A: lane l has dim l % 32, keys 4 (l / 32) + 0..3 and 8 + those of each 16, the
 //                                      order in which S^T leaves them; read transposed from V's rows in LDS
 // 16-bit matrix units, more precise where the types are: a value of more bits is a sum of 16-bit planes, and products
-// of planes whose sum of indexes stays below `depth` are added up (fp32 activations: 3 bf16 planes hold 24 bits; over
-// an fp16 cache 2 fp16 planes of the query scaled into fp16's range hold 22, its weights scaled by 2^14 likewise).
+// of planes whose sum of indexes stays below `depth` are added up.
+//   bf16 activations:           one plane of the query (scaled into fp16's range over fp16 and fp32 caches) and one of
+//                               the weights: rounded to 8 or 11 bits, no more than the output's own rounding
+//   fp32 over a bf16 cache:     3 bf16 planes of the query and the weights hold 24 bits
+//   fp32 over an fp16 cache:    2 fp16 planes hold 22; the query is scaled by a power of two so that its largest value
+//                               is near 2^14, the weights by 2^6 (and 2^kSlack while the maximum lags): what is below
+//                               2^-24 of fp16's scale is lost, 2^-30 of a row's largest weight
+//   fp32 caches (tile kernel):  2 fp16 planes of keys and values, too, each row with its own power of two
+//   fp32 caches (few rows):     fp32 matrix instructions; HBM bounds them all the same
+// Three plane products at 1,100 TFLOP/s beat one at the fp32 units' 154.
 #include <cmath>
 
 #include "page_common.h"
@@ -106,6 +118,16 @@ __device__ __forceinline__ void split2_scaled(float x, float y, float scale, uns
     const halfx2 a = {(_Float16)fmaf(x, scale, 0.f), (_Float16)fmaf(y, scale, 0.f)};
     const halfx2 b = {(_Float16)fmaf(x, scale, -(float)a.x), (_Float16)fmaf(y, scale, -(float)a.y)};
     out[0] = __builtin_bit_cast(unsigned, a);
+    out[1] = __builtin_bit_cast(unsigned, b);
+}
+
+// The same of the values themselves; `one` is 1, and the compiler not to know it.
+__device__ __forceinline__ void split2_mixed(float x, float y, float one, unsigned* out) {
+    const halfx2 a = {(_Float16)x, (_Float16)y};
+    out[0] = __builtin_bit_cast(unsigned, a);
+    asm("" : "+v"(out[0]));  // (not converted a second time for the difference)
+    const halfx2 c = __builtin_bit_cast(halfx2, out[0]);
+    const halfx2 b = {(_Float16)fmaf(x, one, -(float)c.x), (_Float16)fmaf(y, one, -(float)c.y)};
     out[1] = __builtin_bit_cast(unsigned, b);
 }
 
@@ -417,6 +439,17 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// ---- the tile kernel ---------------------------------------------------------------------------------------------
+// 128 packed rows a block, 32 a wavefront; keys and values of a tile (64 keys; 32 of several planes) in LDS, twice, so
+// that one barrier a tile is enough: 66 KB, two blocks a CU, whose matrix and vector instructions fill each other's
+// gaps.  (Tiles of 32 keys and three blocks a CU: 795 us against 709, at the same state of the rest.)  The staged loads
+// of the tile after the next are in flight across the barrier.  The maximum may lag by 2^kSlack, so that most tiles
+// rescale nothing, and the weights of one half of a tile are computed under the other half's matrix instructions.
+// Measured, 32 / 8 heads of 128: bf16, three chunks of 2,048 tokens over 8,192 rows: 657 us, 910 TFLOP/s (a library
+// product of 8192^3: 1,144), matrix units busy for two fifths of the time, the vector units for as much, the rest waits
+// at barriers and for LDS; fp32 over fp16, three chunks of 1,024 tokens: 606 us, 451 TFLOP/s of the formula, twice that
+// of planes.  fp32 rows, 16 / 8 heads, 509 tokens over 1,530 rows: 45 us, of which the parts' way through memory and
+// their merge take a third; over 8,698 rows 149 us, 3.7 us a tile of 32 keys and pair of blocks.
 template <int HD, typename QT, typename KT>
 struct TileSpace {
     typedef Shape<HD, QT, KT> C;
@@ -667,6 +700,8 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         }
     }
 
+    float one = 1.f;
+    asm volatile("" : "+s"(one));
     unsigned long long miss_next = 0;
     if (t0 < t1) {
         load_pages(t0 + 1);
@@ -688,18 +723,27 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         const char* const kbuf = lds + 2 * odd * C::TILE;
         const char* const vbuf = kbuf + C::TILE;
         floatx16 s[KT32];
-        auto scores = [&](int kt) __attribute__((always_inline)) {
+        // LDS reads run ahead of the matrix instructions that take them, by several where one takes 32 cycles (three
+        // chunks of 1,024 tokens, bf16: 425 us one ahead, 406 so; several planes: 625 us, more ahead 643, registers).
+        // kPinned: both keep their order across a step, all else may move.
+        constexpr int kPinned = 0x406, kAhead = NQ == 1 ? 4 : 1, kAheadV = NQ == 1 ? 2 : 1;
+        auto scores = [&]() __attribute__((always_inline)) {  // (caches of one plane)
+            u32x4 kf[kAhead];
+            auto load = [&](int n) __attribute__((always_inline)) {
+                kf[n % kAhead] = *reinterpret_cast<const u32x4*>(kbuf + n / KS * 32 * HD * 2 + (kaddr ^ (n % KS * 32)));
+            };
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[kt][r] = 0.f;
+            for (int n = 0; n < kAhead; n++) load(n);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
+            for (int n = 0; n < KT32 * KS; n++) {
+                if (n % KS == 0)
 #pragma unroll
-                for (int j = 0; j < NK; j++) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + j * C::PLANE + kt * 32 * HD * 2 + (kaddr ^ (ks * 32)));
+                    for (int r = 0; r < 16; r++) s[n / KS][r] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < NQ; i++)
-                        if (i + j < C::DEPTH) s[kt] = E::mac(kf, qf[i][ks], s[kt]);
-                }
+                for (int i = 0; i < NQ; i++) s[n / KS] = E::mac(kf[n % kAhead], qf[i][n % KS], s[n / KS]);
+                if (n + kAhead < KT32 * KS) load(n + kAhead);
+                __builtin_amdgcn_sched_barrier(kPinned);
+            }
         };
         if constexpr (C::KF) {
             // the next tile's planes are made under this one's matrix instructions
@@ -756,33 +800,41 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
             return (sum[0] + sum[1]) + (sum[2] + sum[3]);
         };
         auto products = [&](int kt, float scale) __attribute__((always_inline)) {  // (scale: of fp32 caches)
+            constexpr int N = 2 * NJ * NK;
+            u32x4 vf[kAheadV];
+            auto load = [&](int n) __attribute__((always_inline)) {
+                const int k2 = n / (NJ * NK), jt = n / NK % NJ, j = n % NK;
+                const char* a = vbuf + j * C::PLANE + (vaddr ^ (jt * 64)) + (32 * kt + 16 * k2) * (HD * 2);
+                typedef __attribute__((address_space(3))) shortx4 lds4;
+                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a));
+                const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(a + 8 * HD * 2)));
+                vf[n % kAheadV] = quad(x.x, x.y, y.x, y.y);
+            };
 #pragma unroll
-            for (int k2 = 0; k2 < 2; k2++) {
-                if (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // one step's planes at a time: registers
-                unsigned u[4][NQ];
+            for (int n = 0; n < kAheadV; n++) load(n);
+            u32x4 pf[NQ];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float x = s[kt][8 * k2 + 2 * i], y = s[kt][8 * k2 + 2 * i + 1];
-                    if constexpr (!C::KF) split2<C::F16, NQ, false>(x, y, u[i]);
-                    else if constexpr (NQ == 1) split2<true, 1, false>(x * scale, y * scale, u[i]);
-                    else split2_scaled(x, y, scale, u[i]);
-                }
-                u32x4 pf[NQ];
+            for (int n = 0; n < N; n++) {
+                const int k2 = n / (NJ * NK), jt = n / NK % NJ, j = n % NK;
+                if (n % (NJ * NK) == 0) {
+                    if (NQ > 1 && n) __builtin_amdgcn_sched_barrier(0);  // one step's planes at a time: registers
+                    unsigned u[4][NQ];
 #pragma unroll
-                for (int n = 0; n < NQ; n++) pf[n] = quad(u[0][n], u[1][n], u[2][n], u[3][n]);
-#pragma unroll
-                for (int jt = 0; jt < NJ; jt++)
-#pragma unroll
-                    for (int j = 0; j < NK; j++) {
-                        const char* a = vbuf + j * C::PLANE + (vaddr ^ (jt * 64)) + (32 * kt + 16 * k2) * (HD * 2);
-                        typedef __attribute__((address_space(3))) shortx4 lds4;
-                        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a));
-                        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(a + 8 * HD * 2)));
-                        const u32x4 vf = quad(x.x, x.y, y.x, y.y);
-#pragma unroll
-                        for (int i = 0; i < NQ; i++)
-                            if (i + j < C::DEPTH) o[jt] = E::mac(vf, pf[i], o[jt]);
+                    for (int i = 0; i < 4; i++) {
+                        const float x = s[kt][8 * k2 + 2 * i], y = s[kt][8 * k2 + 2 * i + 1];
+                        if constexpr (!C::KF && C::F16 && NQ == 2) split2_mixed(x, y, one, u[i]);
+                        else if constexpr (!C::KF) split2<C::F16, NQ, false>(x, y, u[i]);
+                        else if constexpr (NQ == 1) split2<true, 1, false>(x * scale, y * scale, u[i]);
+                        else split2_scaled(x, y, scale, u[i]);
                     }
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) pf[q] = quad(u[0][q], u[1][q], u[2][q], u[3][q]);
+                }
+#pragma unroll
+                for (int i = 0; i < NQ; i++)
+                    if (i + j < C::DEPTH) o[jt] = E::mac(vf[n % kAheadV], pf[i], o[jt]);
+                if (n + kAheadV < N) load(n + kAheadV);
+                __builtin_amdgcn_sched_barrier(kPinned);
             }
         };
 
@@ -793,8 +845,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
             if (miss_here == 0 && k0 + BK - 1 <= lim0 && !bad) {
                 const float mu = m - C::BIAS;
                 if (NQ > 1) __builtin_amdgcn_s_setprio(1);  // (several planes: matrix instructions first)
-                scores(0);
-                if constexpr (KT32 > 1) scores(1);
+                scores();
                 if (NQ > 1) __builtin_amdgcn_s_setprio(0);
                 float mx = largest(0);
                 float sum = weights(0, mu);
@@ -813,8 +864,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
             }
         }
         if constexpr (!C::KF) {
-#pragma unroll
-            for (int kt = 0; kt < KT32; kt++) scores(kt);
+            scores();
         } else {
 #pragma unroll
             for (int kt = 0; kt < KT32; kt++)
@@ -940,6 +990,9 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
 // fp32 ones do not: v_mfma_f32_16x16x4_f32 wants one value of a key per lane, and output row i of tile (a, j) is dim
 // 64 a + 4 i + j, so that 16 bytes of a value row feed four tiles.  Of the next tile, keys are loaded when this one's
 // scores are done and values when its own are in LDS (or used).
+// HBM bounds it.  Measured, head size 128: 16 sequences of up to 8,192 rows (386 MB, fp16): 78 us, 4.95 TB/s, what a
+// large copy reaches; 8 of 4,000 fp32 rows (194 MB): 46 us, 4.2 TB/s; one of 4,096 rows (17 MB): 14 us, of which two
+// launches and the wait for the first keys are 10; one token over 100 rows: 7 us, a launch and its dependent loads.
 template <int HD>
 struct FewSpace {
     char lds[kWaves * 32 * HD * 2];  // values, later the wavefronts' outputs
@@ -1267,7 +1320,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedParam
 }
 
 // ---- the splits of a row, in a fixed order ------------------------------------------------------------------------
-// A block takes 16 rows of a tile; where a tile has fewer, several groups of HD / 4 lanes share a row's splits.
+// A block takes 16 rows of a tile; where a tile has fewer, several groups of HD / 4 lanes share a row's splits.  Bound by
+// memory (the parts come out of L2 and the cache behind it): 5.3 us after the decode step above, 8.9 us for the 29 MB of
+// the fp32 chunk's.
 template <int HD, typename QT, int ROWS>
 __device__ __forceinline__ void merge_block(const PagedParams& p, int b, int kvh, float (*s_o)[HD], float* s_l) {
     constexpr int LPR = HD / 4, NG = 512 / LPR;
@@ -1332,9 +1387,12 @@ struct Part {
     }
 };
 
-// The launches of a call.  The host knows the numbers of rows and of chunks, not which chunk has how many: where the
-// rows are few for the chunks every chunk goes to the few-row kernel, where there is one chunk of many rows it goes to
-// the tile kernel, otherwise both are launched and share the chunks by their rows.
+// The launches of a call.  The host knows the numbers of rows and of chunks, not which chunk has how many.  Up to 32
+// packed rows a chunk on average, all chunks go to the few-row kernel (16 sequences, 8 tokens, 4 heads a KV head, 22 rows
+// on average: 36 us, tiles 46; 16 tokens, 45 rows: 49 us, tiles 39).  One chunk of more rows goes to the tile kernel.
+// Otherwise one launch holds both kernels' blocks, and chunks of up to kFewRows rows are the few-row kernel's (decode
+// steps and a prompt together, fp16 and fp32: 143 and 290 us, all as tiles 162 and 338; kFewRows 64 instead of 16: 16
+// chunks of 16 tokens 53 us instead of 39 in bf16, 63 instead of 44 in fp32).
 struct Plan {
     int few_rows = 0;  // packed rows up to which a chunk is the few-row kernel's
     Part few, tile;
@@ -1359,7 +1417,8 @@ int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int he
     AR_CHECK_ARG(packed <= 1 << 30 && (packed / 16 + c->n) * p->kv_heads < 1 << 23, "paged attention: %d rows of %d heads are too many",
                  c->rows, heads);
     Plan a;
-    // (fp32 rows keep twice the bytes in flight: one block a CU was enough; 16-bit caches and tiles: two)
+    // (Few rows over fp32, which keep twice the bytes in flight: one block a CU, 46 us for 8 sequences of 4,000 rows, two
+    // 52; 16-bit caches: two, 82 us for 16 of 8,192, one 88.  Tiles: two, 46 us for the fp32 chunk, one 52.)
     const int few_cu = p->dtype == AR_DTYPE_F32 ? 1 : 2, tile_cu = 2;
     if (!c->start || packed <= 32LL * c->n) {
         a.few_rows = 0x7fffffff;

@@ -8,6 +8,8 @@
 // thread holds the dims f .. f+3 and f + hd/2 .. +3 of a head, so a 16-byte load each feeds its four rotations, a head
 // is hd / 8 lanes of one wavefront, and its norm is a reduction within them.  Angles: hd / 2 per row and not per head,
 // computed by the block's first threads in double (a position times a frequency, less whole turns) and shared in LDS.
+// Measured: 6,958 rows of 16 / 8 heads of 128 to bf16 (171 MB) 31 us, 5.5 TB/s; a decode step of 8 rows 5 us, a launch
+// and its chain of loads (chunk, page, angles).
 #include <cmath>
 
 #include "page_common.h"
