@@ -5,6 +5,7 @@ The compute path is the native library ``common_amd/lib/libar_hip.so`` (C-ABI in
 
 * ``hardware``  -- context / memory provider / operators (the backend SPI objects)
 * ``qwen3``     -- Qwen3 + AutoregressiveModel token loop
+* ``pages``     -- paged KV cache for serving many sequences: page calls, row preparation, attention
 * ``config``    -- Qwen3Config and the benchmark configurations
 * ``synthetic`` -- seeded synthetic weights and prompts
 """
