@@ -186,8 +186,9 @@ template <>
 struct Kind<_Float16> { static constexpr int id = AR_DTYPE_F16; };
 
 constexpr int kThreads = 256, kWaves = 4;
-// The tile kernel's maximum of a row may lag behind by this power of two: weights up to 2^kSlack (fp16: 2^14).
-constexpr float kSlack = 8.f;
+// The tile kernel's maximum of a row may lag behind by this power of two: weights up to 2^kSlack (fp16: 2^14); what a
+// lane's weights of a tile may add up to without a look at their maximum.
+constexpr float kSlack = 8.f, kBound = 16384.f;
 
 // Planes and sizes of a (head size, activation, cache) combination.
 template <int HD, typename QT, typename KT>
@@ -444,7 +445,7 @@ __device__ __forceinline__ void lds_barrier() {
 // that one barrier a tile is enough: 66 KB, two blocks a CU, whose matrix and vector instructions fill each other's
 // gaps.  (Tiles of 32 keys and three blocks a CU: 795 us against 709, at the same state of the rest.)  The staged loads
 // of the tile after the next are in flight across the barrier.  The maximum may lag by 2^kSlack, so that most tiles
-// rescale nothing, and the weights of one half of a tile are computed under the other half's matrix instructions.
+// rescale nothing.  (The second half's weights under the first one's matrix instructions: the same time.)
 // Measured, 32 / 8 heads of 128: bf16, three chunks of 2,048 tokens over 8,192 rows: 657 us, 910 TFLOP/s (a library
 // product of 8192^3: 1,144), matrix units busy for two fifths of the time, the vector units for as much, the rest waits
 // at barriers and for LDS; fp32 over fp16, three chunks of 1,024 tokens: 606 us, 451 TFLOP/s of the formula, twice that
@@ -791,11 +792,11 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         };
         // scores to weights; their sum, of this lane's half of the keys
         auto weights = [&](int kt, float mu) __attribute__((always_inline)) {
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float sum[4];
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], c, -mu));
-                sum[r & 3] += s[kt][r];
+                sum[r & 3] = r < 4 ? s[kt][r] : sum[r & 3] + s[kt][r];
             }
             return (sum[0] + sum[1]) + (sum[2] + sum[3]);
         };
@@ -839,28 +840,26 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         };
 
         if (k0 > lim1) continue;
-        // Tiles that every row sees in full, while no row's scores pass its maximum by much (most of them): the weights of
-        // a half are computed under the matrix instructions of the other half.
+        // Tiles that every row sees in full, while no row's weights pass a bound (most of them): their sum, which every
+        // weight is below, is all that is looked at.  (No key seen before: infinity; NaN passes no bound.)
+        float slack = kSlack;
         if constexpr (!C::KF) {
             if (miss_here == 0 && k0 + BK - 1 <= lim0 && !bad) {
-                const float mu = m - C::BIAS;
                 if (NQ > 1) __builtin_amdgcn_s_setprio(1);  // (several planes: matrix instructions first)
                 scores();
                 if (NQ > 1) __builtin_amdgcn_s_setprio(0);
-                float mx = largest(0);
-                float sum = weights(0, mu);
-                if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
-                if (!__ballot(!(fmaf(mx, c, -m) <= kSlack))) {  // (no key seen yet: NaN or infinity)
+                float sum = 0.f;
+#pragma unroll
+                for (int kt = 0; kt < KT32; kt++) sum += weights(kt, m - C::BIAS);
+                if (!__ballot(!(sum <= kBound))) {
+                    l += sum;
                     if (NQ > 1) __builtin_amdgcn_s_setprio(1);
                     products(0, 1.f);
                     if (NQ > 1) __builtin_amdgcn_s_setprio(0);
-                    if constexpr (KT32 > 1) {
-                        sum += weights(1, mu);
-                        products(1, 1.f);
-                    }
-                    l += sum;
+                    if constexpr (KT32 > 1) products(1, 1.f);
                     continue;
                 }
+                slack = 0.f;
             }
         }
         if constexpr (!C::KF) {
@@ -893,7 +892,7 @@ __device__ __forceinline__ void tile_block(const PagedParams& p, int index, int 
         float mx = largest(0);
         if constexpr (KT32 > 1) mx = fmaxf(mx, largest(1));
         mx = max_xor32(mx) * c;
-        if (__ballot(mx - m > kSlack)) {  // (no key seen before: infinity; none yet: NaN)
+        if (__ballot(mx - m > slack)) {  // (no key seen before: infinity; none yet: NaN)
             const float mn = fmaxf(m, mx);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= alpha;
