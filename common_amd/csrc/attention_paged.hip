@@ -441,16 +441,16 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // ---- the tile kernel ---------------------------------------------------------------------------------------------
-// 128 packed rows a block, 32 a wavefront; keys and values of a tile (64 keys; 32 of several planes) in LDS, twice, so
+// 128 packed rows a block, 32 a wavefront; keys and values of a tile (64 keys; 32 of fp32 rows or three planes) in LDS, twice, so
 // that one barrier a tile is enough: 66 KB, two blocks a CU, whose matrix and vector instructions fill each other's
 // gaps.  (Tiles of 32 keys and three blocks a CU: 795 us against 709, at the same state of the rest.)  The staged loads
 // of the tile after the next are in flight across the barrier.  The maximum may lag by 2^kSlack, so that most tiles
 // rescale nothing.  (The second half's weights under the first one's matrix instructions: the same time.)
 // Measured, 32 / 8 heads of 128: bf16, three chunks of 2,048 tokens over 8,192 rows: 657 us, 910 TFLOP/s (a library
-// product of 8192^3: 1,144), matrix units busy for two fifths of the time, the vector units for as much, the rest waits
-// at barriers and for LDS; fp32 over fp16, three chunks of 1,024 tokens: 606 us, 451 TFLOP/s of the formula, twice that
-// of planes.  fp32 rows, 16 / 8 heads, 509 tokens over 1,530 rows: 45 us, of which the parts' way through memory and
-// their merge take a third; over 8,698 rows 149 us, 3.7 us a tile of 32 keys and pair of blocks.
+// product of 8192^3: 1,144); matrix units busy for 40% of the time, vector units for 36%, little of it at once:
+// wavefronts wait to issue for 36%.  fp32 over fp16, three chunks of 1,024 tokens: 597 us, 457 TFLOP/s of the formula,
+// twice that of planes.  fp32 rows, 16 / 8 heads, 509 tokens over 1,530 rows: 45 us, of which the parts' way through
+// memory and their merge take a third; over 8,698 rows 149 us, 3.7 us a tile of 32 keys and pair of blocks.
 template <int HD, typename QT, typename KT>
 struct TileSpace {
     typedef Shape<HD, QT, KT> C;

@@ -10,8 +10,8 @@ constexpr int kMaxEntries = 4096;  // chunks / entries of one table call: their 
 // Bound by HBM, each byte read and written once.  A block moves pieces of 16 KB: 256 threads x four 16-byte loads in
 // flight before their stores, so 8 blocks on a CU keep 128 KB in flight.  Measured: 255 pages of 28 layers (1.87 GB read
 // and written) 380 us, 4.9 TB/s, what one large copy reaches; 9 small pages 6 us, a launch; four pages of 48 KB in each
-// of 12 layers 17 us: they lie at the same place in every layer, so that few memory channels serve them all.  2 to 16
-// blocks a CU make no difference.
+// of 12 layers 17 us (a constant distance apart: most likely few memory channels serve them all).  2 to 16 blocks a CU
+// make no difference.
 constexpr int kCopyThreads = 256, kCopyUnroll = 4, kPieceBytes = 16384;
 
 struct CopyParams {

@@ -133,7 +133,7 @@ int ar_hip_pages_write(ar_hip_ctx *ctx, const ar_pages *pages, int layer, const 
  * caches, to the largest value of its row of the cache over fp32 ones, and what a weight of less than 2^-30 of its
  * row's largest loses is below 2^-30 of the value that it weighs.  With bf16 activations the softmax weights are
  * rounded to 16 bits (the cache's type; fp16 for fp32 caches) for the second product.
- * (chunks->rows * heads is at most 2^27, and no more than 2^23 tiles of 16 packed rows.) */
+ * chunks->rows * heads / 16 + chunks->n * kv_heads must be below 2^23. */
 int ar_hip_attention_paged_work(ar_hip_ctx *ctx, const ar_pages *pages, const ar_chunks *chunks, int heads,
                                 size_t *bytes);
 int ar_hip_attention_paged(ar_hip_ctx *ctx, const ar_pages *pages, int layer, const ar_chunks *chunks, const void *q,

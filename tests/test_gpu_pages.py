@@ -11,6 +11,9 @@ fp16 2^-11):
 Table calls and copies are exact.
 """
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -912,3 +915,142 @@ def test_serving_loop_matches_whole_sequences(ctx, act, dtype):
     cache.close()
     for x in (gqd, gkd, ms):
         x.free()
+
+
+def test_offsets_past_32_bits(ctx):
+    """The second layer of pools of 5.2 GB: rows written to the last pages, moved by a copy, attended to from one
+    token and from a chunk."""
+    r = _rng(83)
+    KV, hd, P, pages, H = 8, 128, 64, 20000, 16
+    lengths, counts = [190, 300], [1, 70]
+    cache = pg.PagedCache(ctx, 2, pages, KV, hd, 2, 6, page_rows=P, dtype=CODE["bf16"])
+    table = np.full((2, 6), -1, np.int32)
+    table[0, :3], table[1, :5] = [19990, 19999, 19985], [19980, 19998, 19970, 19991, 19960]
+    td = ctx.to_device(table)
+    moved = [19998, 19985]
+    rows = sum(lengths)
+    k, v = (r.standard_normal((rows, KV, hd)).astype(np.float32) for _ in range(2))
+    kd, vd, at, st = ctx.to_device(k), ctx.to_device(v), _i32(ctx, [0, 0]), _i32(ctx, _starts(lengths))
+    cache.raw.table = td.ptr
+    cache.write(1, pg.Chunks(2, rows, at=at, start=st), None, kd, vd, None, H, pg.Rotary(1e6, None, [hd // 2]))
+    pos = np.concatenate([np.arange(n) for n in lengths])[None]
+    pk = ref.values(ref.to_bits(ref.prepared(k, None, 0, True, pos, np.zeros(hd // 2, int), 1e6), "bf16"))
+    pv = ref.values(ref.to_bits(v, "bf16"))
+    q = r.standard_normal((sum(counts), H, hd))
+    host = ref.to_bits(q, "bf16")
+    qd, od = ctx.to_device(host), ctx.allocate(host.nbytes)
+    first = [n - c for n, c in zip(lengths, counts)]
+    at2, st2 = _i32(ctx, first), _i32(ctx, _starts(counts))
+    src, dst = _i32(ctx, moved), _i32(ctx, [3, 19997])
+    outs = []
+    for step in range(2):
+        if step:
+            cache.copy(cache, src, dst, 2)
+            t2 = table.copy()
+            t2[table == moved[0]], t2[table == moved[1]] = 3, 19997
+            ctx.synchronize()
+            td.upload(t2)
+        for i in (0, 1):  # one token, then the chunk (few rows, then tiles)
+            one = pg.Chunks(1, counts[i], at=_At(at2, i), start=_At(st2, 0) if i == 0 else _i32(ctx, [0, counts[1]]),
+                            seq=_i32(ctx, [i]))
+            row = sum(counts[:i]) * H * hd * 2
+            cache.attention(1, one, _At(qd, row // 4), _At(od, row // 4), H, CODE["bf16"])
+        ctx.synchronize()
+        outs.append(ref.values(od.download(np.uint16, host.size).reshape(host.shape)))
+    np.testing.assert_array_equal(outs[0], outs[1])
+    qv, ks, cs = ref.values(host), _starts(lengths), _starts(counts)
+    for i in range(2):
+        known = np.ones(lengths[i], bool)
+        kk, vv = pk[ks[i]:ks[i + 1]], pv[ks[i]:ks[i + 1]]
+        (out, mag, big), = ref.attention([qv[cs[i]:cs[i + 1]]], [(kk, known)], [(vv, known)], [first[i]], [counts[i]], H)
+        half, step_k = HALF_STEP["bf16"], 2 * HALF_STEP["bf16"] / 8  # (keys near the middle of two stored values)
+        tol = (64 * U * big + 32 * U + half + step_k * big) * mag + half * np.abs(out)
+        assert (np.abs(outs[0][cs[i]:cs[i + 1]] - out) <= tol).all()
+    cache.close()
+
+
+class _At:
+    """A buffer's int32 at an index."""
+
+    def __init__(self, buf, index):
+        self.ptr = buf.ptr + 4 * index
+
+
+def test_grow_and_write_with_chunk_starts_of_anything_stay_inside(ctx):
+    """Starts that descend or leave the rows make empty chunks; nothing outside the sequences' pages changes."""
+    r = _rng(89)
+    for starts in ([0, 10, 5, 20, 40], [0, 10, 90, 95, 99], [-7, 3, 20, 2 ** 31 - 1, 9], [0, 40, 0, 40, 0]):
+        pool = Pool(ctx, r, "f32", 1, 1, 64, 16, [20, 7, 0, 33], cols=8, spare=20)
+        t = _tables(pool)
+        counts = [b - a if a >= 0 and b > a and b <= 40 else 0 for a, b in zip(starts, starts[1:])]
+        at, st, ms = _i32(ctx, [-5] * 4), _i32(ctx, starts), _i32(ctx, [-5])
+        ch = pg.Chunks(4, 40, at=at, start=st)
+        pool.cache.grow(ch, ms)
+        want, missing = t.grow(range(4), counts)
+        np.testing.assert_array_equal(at.download(np.int32, 4), want)
+        assert ms.download(np.int32, 1)[0] == missing
+        _same(pool, t)
+        x = [ctx.to_device(r.standard_normal((40, n, 64)).astype(np.float32)) for n in (2, 1, 1, 2)]
+        pool.cache.write(0, ch, x[0], x[1], x[2], x[3], 2, pg.Rotary(1e4, None, [32]))
+        ctx.synchronize()
+        free = pool.refs == 0
+        for name in ("k", "v"):
+            np.testing.assert_array_equal(pool.down(name)[:, free], getattr(pool, name)[:, free])
+            got = pool.down(name)
+            for s, n in enumerate([20, 7, 0, 33]):  # rows that were there before
+                for row in range(n):
+                    page = pool.table[s, row // 16]
+                    np.testing.assert_array_equal(got[0, page, :, row % 16], getattr(pool, name)[0, page, :, row % 16])
+        pool.free()
+        for b in x + [at, st, ms]:
+            b.free()
+
+
+CHILD = r"""
+import ctypes, sys
+sys.path.insert(0, ROOT)
+import numpy as np
+from common_amd import hardware as hw, pages as pg
+with hw.HipContext(0) as ctx:
+    i32 = lambda v: ctx.to_device(np.asarray(v, np.int32))
+    H, KV, hd = 4, 2, 64
+    with pg.PagedCache(ctx, 2, 12, KV, hd, 3, 5, page_rows=16) as cache, pg.PagedCache(ctx, 2, 9, KV, hd, 0, 0, page_rows=16) as other:
+        at, st, ms = i32([-1, -1]), i32([0, 40, 45]), i32([0])
+        ch = pg.Chunks(2, 45, at=at, start=st)
+        q, k, v, o = (ctx.to_device(np.ones((45, n, hd), np.float32)) for n in (H, KV, KV, H))
+        cache.grow(ch, ms)
+        cache.write(0, ch, q, k, v, q, H, pg.Rotary(1e4, i32(np.zeros(90)), [20, 12]))
+        cache.attention(0, ch, q, o, H)
+        cache.fork(i32([0]), i32([2]), 1)
+        cache.trim(i32([1]), i32([2]), 1)
+        cache.compact(ms)
+        cache.copy(other, i32([0]), i32([1]), 1)
+        ctx.synchronize()
+        n = ctypes.c_ulonglong()
+        hw.check(hw.lib().ar_hip_pointer_checks(ctypes.byref(n)))
+        print("checked", n.value)
+        short = ctx.allocate(44 * H * hd * 4)
+        # (the last int32 of a whole number of 4 KB: HIP gives a few bytes a longer range than was asked for)
+        class end: ptr = short.ptr + 44 * H * hd * 4 - 4
+        for call in (lambda: cache.attention(0, ch, q, short, H), lambda: cache.attention(0, ch, short, o, H),
+                     lambda: cache.write(0, ch, q, short, v, q, H, pg.Rotary(1e4, None, [32]), kv_stride=H * hd),
+                     lambda: cache.write(0, ch, q, k, v, q, H, pg.Rotary(1e4, i32(np.zeros(44)), [32])),
+                     lambda: cache.trim(end, end, 2)):
+            try:
+                call()
+                print("passed")
+            except Exception as e:
+                print("refused", "leaves its allocation" in str(e))
+        ctx.synchronize()
+"""
+
+
+def test_pointer_checks_cover_the_paged_calls():
+    """AR_HIP_CHECK_PTRS=1 (read once per process: a child): every call passes, and is refused when a buffer is short."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", "ROOT = %r\n" % root + CHILD], env=dict(os.environ, AR_HIP_CHECK_PTRS="1"),
+                       capture_output=True, text=True, timeout=110)
+    assert p.returncode == 0, p.stderr[-3000:]
+    lines = p.stdout.split("\n")
+    assert lines[0].startswith("checked") and int(lines[0].split()[1]) > 40, p.stdout
+    assert lines[1:6] == ["refused True"] * 5, p.stdout
