@@ -29,13 +29,15 @@ struct CopyParams {
     int s_pages, d_pages, same_pool;
 };
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));  // (an array of structures goes to LDS: 17 us for 4)
+
 __device__ __forceinline__ void copy_run(const char* s, char* d, unsigned bytes) {
     const unsigned units = bytes / 16, step = kCopyThreads * kCopyUnroll;
-    const uint4* a = reinterpret_cast<const uint4*>(s);
-    uint4* b = reinterpret_cast<uint4*>(d);
+    const u32x4* a = reinterpret_cast<const u32x4*>(s);
+    u32x4* b = reinterpret_cast<u32x4*>(d);
     unsigned i = threadIdx.x;
     for (; i + step - kCopyThreads < units; i += step) {
-        uint4 t[kCopyUnroll];
+        u32x4 t[kCopyUnroll];
 #pragma unroll
         for (int u = 0; u < kCopyUnroll; u++) t[u] = a[i + u * kCopyThreads];
 #pragma unroll
