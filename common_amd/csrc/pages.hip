@@ -9,9 +9,9 @@ constexpr int kMaxEntries = 4096;  // chunks / entries of one table call: their 
 // ---- page copies -----------------------------------------------------------------------------------
 // Bound by HBM, each byte read and written once.  A block moves pieces of 16 KB: 256 threads x four 16-byte loads in
 // flight before their stores, so 8 blocks on a CU keep 128 KB in flight.  Measured: 255 pages of 28 layers (1.87 GB read
-// and written) 380 us, 4.9 TB/s, what one large copy reaches; 9 small pages 6 us, a launch; four pages of 48 KB in each
-// of 12 layers 17 us (a constant distance apart: most likely few memory channels serve them all).  2 to 16 blocks a CU
-// make no difference.
+// and written) 371 us, 5.0 TB/s, what one large copy reaches; 16 of them 25 us; 9 small pages 5 us, a launch.  Pieces of 4
+// and 8 KB: 389 and 380 us (16 KB: 381).  Loads and stores that leave the caches to others: 381 -> 371 us, 64 forks'
+// last pages 211 -> 202.
 constexpr int kCopyThreads = 256, kCopyUnroll = 4, kPieceBytes = 16384;
 
 struct CopyParams {
@@ -39,9 +39,9 @@ __device__ __forceinline__ void copy_run(const char* s, char* d, unsigned bytes)
     for (; i + step - kCopyThreads < units; i += step) {
         u32x4 t[kCopyUnroll];
 #pragma unroll
-        for (int u = 0; u < kCopyUnroll; u++) t[u] = a[i + u * kCopyThreads];
+        for (int u = 0; u < kCopyUnroll; u++) t[u] = __builtin_nontemporal_load(a + i + u * kCopyThreads);
 #pragma unroll
-        for (int u = 0; u < kCopyUnroll; u++) b[i + u * kCopyThreads] = t[u];
+        for (int u = 0; u < kCopyUnroll; u++) __builtin_nontemporal_store(t[u], b + i + u * kCopyThreads);
     }
     for (; i < units; i += kCopyThreads) b[i] = a[i];
 }
