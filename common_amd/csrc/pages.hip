@@ -27,6 +27,10 @@ struct CopyParams {
     // or page numbers of the caller's
     const int *src, *dst;
     int s_pages, d_pages, same_pool;
+    // a table whose entries move with the pages (null: none): page g becomes to[g]
+    int* table;
+    const int* to;
+    size_t cells;
 };
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));  // (an array of structures goes to LDS: 17 us for 4)
@@ -47,6 +51,15 @@ __device__ __forceinline__ void copy_run(const char* s, char* d, unsigned bytes)
 }
 
 __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyParams p) {
+    if (p.table) {
+        const size_t step = (size_t)gridDim.x * gridDim.y * kCopyThreads;
+        for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * kCopyThreads + threadIdx.x; i < p.cells; i += step) {
+            const int page = p.table[i];
+            if (page < 0 || page >= p.s_pages) continue;
+            const int to = p.to[page];
+            if (to != page) p.table[i] = to;
+        }
+    }
     const int slots = p.count ? min(*p.count, p.slots) : p.slots;
     for (int slot = blockIdx.y; slot < slots; slot += gridDim.y) {
         int s, d;
@@ -347,11 +360,11 @@ __global__ __launch_bounds__(256) void fork_write_kernel(ForkParams p) {
 }
 
 // ---- compacting --------------------------------------------------------------------------------------------
-// One block ranks holes and movers (5 to 7 us), all blocks rewrite the table, then the pages move: sources and targets
-// are disjoint.  48 sequences of 1,100 rows, a third of them gone: 630 us for 3.1 GB, the copies' rate.
+// One block ranks holes and movers (5 to 6 us), then the copies' blocks rewrite the table and move the pages: sources and
+// targets are disjoint.  48 sequences of 1,100 rows, a third of them gone: 600 us for 3.1 GB, the copies' rate.
 struct CompactParams {
-    int *table, *refs;
-    int seqs, max_pages, pages;
+    int* refs;
+    int pages;
     int* live;
     int2* pairs;  // [pages / 2]: moves
     int* count;   // moves
@@ -403,17 +416,6 @@ __global__ __launch_bounds__(1024) void compact_plan_kernel(CompactParams p) {
     if (tid == 0) {
         *p.count = movers;
         if (p.live) *p.live = live;
-    }
-}
-
-__global__ __launch_bounds__(256) void compact_table_kernel(CompactParams p) {
-    const size_t cells = (size_t)p.seqs * p.max_pages;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (size_t)gridDim.x * 256) {
-        const int page = p.table[i];
-        if (page >= 0 && page < p.pages) {
-            const int to = p.to[page];
-            if (to != page) p.table[i] = to;
-        }
     }
 }
 
@@ -590,20 +592,18 @@ extern "C" int ar_hip_pages_compact(ar_hip_ctx* ctx, const ar_pages* pages, int3
         AR_TRY(ar_check_range(work, work_bytes_of(pages, 0), what, "work space"));
     }
     CompactParams c;
-    c.table = pages->table; c.refs = pages->refs; c.seqs = pages->seqs; c.max_pages = pages->max_pages;
-    c.pages = pages->pages; c.live = live; c.count = (int*)work; c.pairs = (int2*)((char*)work + 16);
+    c.refs = pages->refs; c.pages = pages->pages; c.live = live; c.count = (int*)work; c.pairs = (int2*)((char*)work + 16);
     c.to = (int*)(c.pairs + pages->pages / 2);
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(1024), 0, ctx->stream, c);
     AR_LAUNCH_CHECK();
-    const size_t cells = (size_t)pages->seqs * pages->max_pages;
-    hipLaunchKernelGGL(compact_table_kernel, dim3((unsigned)std::min<size_t>((cells + 255) / 256, 2048)), dim3(256), 0,
-                       ctx->stream, c);
-    AR_LAUNCH_CHECK();
-    if (pages->pages < 2) return AR_HIP_OK;
+    if (pages->pages < 2) return AR_HIP_OK;  // (nothing can move)
     CopyParams m = copy_params(pages, pages);
     m.pairs = c.pairs;
     m.count = c.count;
     m.slots = pages->pages / 2;
+    m.table = pages->table;
+    m.to = c.to;
+    m.cells = (size_t)pages->seqs * pages->max_pages;
     return launch_copy(ctx, m);
 }
 
