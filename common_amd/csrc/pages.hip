@@ -147,7 +147,7 @@ __device__ __forceinline__ int block_prefix(int v, int* part, int* total) {
 // ---- taking pages --------------------------------------------------------------------------------------
 // One block: the chunks' needs, their prefix sum, the free pages in ascending order, then table and counts.  The
 // work is small (a few words per chunk and page); what bounds it is the chain of dependent loads: 6 us for 4 chunks, 9
-// for 128, 10.6 for 16 chunks that take 300 pages.  (Several blocks would need a launch between the steps, 3 us each.)
+// for 128.  (Several blocks would need a launch between the steps, 3 us each.)
 struct GrowParams {
     int *table, *rows, *refs;
     int seqs, max_pages, pages, shift;
