@@ -333,7 +333,7 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         }
         const double inv = 1. / ((double)share * kUnit<ROWS>);
         const int per = (int)fminf(share, 1 << 24);  // (no chunk has more units)
-        int tasks = 0, tiles = 0;  // before this round's chunks
+        int tasks = 0, tiles = 0;  // before these 64 chunks
         bool found = false;
         for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
             if (i0) n = chunk_tiles<ROWS>(p, i0 + lane, &c);

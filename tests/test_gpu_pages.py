@@ -348,6 +348,37 @@ def test_a_first_tile_of_scores_of_minus_infinity(ctx, act, dtype):
     pool.free()
 
 
+@pytest.mark.parametrize("act,dtype", TYPES)
+@pytest.mark.parametrize("slope", [0.02, -0.02, 0.15, 1.0, -1.0])
+@pytest.mark.parametrize("hd,at,counts", [(64, [900], [1]), (128, [500], [70]), (64, [700, 20, 300], [40, 2, 90])])
+def test_scores_that_rise_or_fall_along_the_keys(ctx, act, dtype, slope, hd, at, counts):
+    """Rows of one tile whose scores rise, fall or stay: maxima that lag behind and jump, in some rows of a wavefront."""
+    r = _rng(97)
+    pool = Pool(ctx, r, dtype, 1, 2, hd, 32, [a + c for a, c in zip(at, counts)])
+    k = 0.1 * r.standard_normal(pool.k.shape)
+    for i in range(len(at)):
+        for col, page in enumerate(pool.table[i]):
+            if page >= 0:
+                k[0, page, :, :, 0] = slope * (col * 32 + np.arange(32)) * np.sqrt(hd)
+    pool.set("k", ref.to_bits(k.astype(np.float32), dtype))
+    q = 0.5 * r.standard_normal((sum(counts), 8, hd))
+    q[..., 0] = r.choice([1.0, 0.0, -1.0, 0.3], q.shape[:2])
+    got = _attend(ctx, pool, 0, at, counts, q, act, 8)
+    _check_attention(got, pool, 0, at, counts, q, act, 8)
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("at,counts", [([60, 63], [3, 1]), ([40], [90]), ([64, 2 ** 31 - 1, 0], [70, 2, 100])])
+def test_rows_past_the_table_see_all_of_it(ctx, act, dtype, at, counts):
+    r = _rng(101)
+    pool = Pool(ctx, r, dtype, 1, 2, 64, 16, [64] * len(at))
+    q = r.standard_normal((sum(counts), 4, 64))
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    _check_attention(got, pool, 0, at, counts, q, act, 4)
+    pool.free()
+
+
 @pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("case", ["ones", "ones-starts", "mixed", "slots-few", "slots-mixed"])
 def test_attention_of_many_chunks(ctx, act, dtype, case):
@@ -412,6 +443,35 @@ def test_attention_in_place(ctx, act, dtype, at, counts):
     ctx.synchronize()
     np.testing.assert_array_equal(ref.values(qd.download(host.dtype, host.size).reshape(host.shape)), apart)
     for b in (qd, ad, sd):
+        b.free()
+    pool.free()
+
+
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("at,counts", [([3000, 20, -1], [1, 1, 1]), ([600], [150]), ([10, 1500, 900, 0], [90, 1, 30, 0])])
+def test_what_the_work_space_held_means_nothing(ctx, act, dtype, at, counts):
+    r = _rng(103)
+    pool = Pool(ctx, r, dtype, 1, 2, 128, 64, [max(a, 0) + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), 8, 128))
+    host = ref.to_bits(q, act)
+    ad, sd, qd = _i32(ctx, at), _i32(ctx, _starts(counts)), ctx.to_device(host)
+    ch = pg.Chunks(len(counts), len(q), at=ad, start=sd)
+    need = ctypes.c_size_t()
+    hw.check(hw.lib().ar_hip_attention_paged_work(ctx.handle, pool.cache.ref, ch.ref, 8, ctypes.byref(need)))
+    got = []
+    for fill in (0, 0xFFFFFFFF, 0x7F7FFFFF):  # zeros, NaN, the largest float
+        w = ctx.to_device(np.full(-(-need.value // 4), fill, np.uint32))
+        od = ctx.allocate(host.nbytes)
+        hw.check(hw.lib().ar_hip_attention_paged(ctx.handle, pool.cache.ref, 0, ch.ref, qd.ptr, CODE[act], 8, od.ptr, w.ptr,
+                                                 need.value))
+        ctx.synchronize()
+        got.append(ref.values(od.download(host.dtype, host.size).reshape(host.shape)))
+        w.free()
+        od.free()
+    np.testing.assert_array_equal(got[0], got[1])
+    np.testing.assert_array_equal(got[0], got[2])
+    _check_attention(got[0], pool, 0, at, counts, q, act, 8)
+    for b in (ad, sd, qd):
         b.free()
     pool.free()
 
