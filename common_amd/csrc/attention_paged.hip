@@ -56,6 +56,7 @@ struct PagedParams {
     int heads, kv_heads, group, seqs, max_pages, pages, shift, n, rows;
     float scale;          // log2(e) / sqrt(head_dim)
     int few_rows;         // chunks of at most this many packed rows are the few-row kernel's
+    int merge_rows;       // of a tile, that a merging block takes
     PartArgs few, tile;
 };
 
@@ -1319,57 +1320,66 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedParam
 }
 
 // ---- the splits of a row, in a fixed order ------------------------------------------------------------------------
-// A block takes 16 rows of a tile; where a tile has fewer, several groups of HD / 4 lanes share a row's splits.  Bound by
-// memory (the parts come out of L2 and the cache behind it): 5.3 us after the decode step above, 8.9 us for the 29 MB of
-// the fp32 chunk's.
+// A block takes 16 rows of a tile, or twice 16 where that many blocks would not be resident at once (16 chunks of 64
+// tokens in bf16: 62.4 us, 64.6 with 16; 509 fp32 tokens of one chunk: 48.3 and 47.5); where there are fewer rows, several
+// groups of HD / 4 lanes share a row's splits.  Bound by memory (the parts come out of L2 and the cache behind it) and by
+// the way to its task: 5.4 us after the decode step above, 8.6 us for the 29 MB of the fp32 chunk's.
 template <int HD, typename QT, int ROWS>
 __device__ __forceinline__ void merge_block(const PagedParams& p, int b, int kvh, float (*s_o)[HD], float* s_l) {
     constexpr int LPR = HD / 4, NG = 512 / LPR;
+    const int per_block = ROWS == 16 ? 16 : p.merge_rows, blocks = ROWS / per_block;
     const PartArgs& a = ROWS == 16 ? p.few : p.tile;
-    const int r0 = 16 * (b % (ROWS / 16));
     Task found;
-    if (!find_task<ROWS, true>(p, b / (ROWS / 16), &found)) return;
+    if (!find_task<ROWS, true>(p, b / blocks, &found)) return;
     const Task t = settled(found);
     // (chunks whose starts are not in order may have more tasks than there is space for: they are not all computed)
     if (t.splits == 1 || t.base < 0 || t.base + t.splits > a.tasks) return;
-    const int rows = min(t.rows - r0, 16);
-    if (rows <= 0) return;
-    int share = 1;  // groups of a row
-    while (2 * share * rows <= NG) share *= 2;
-    const int group = threadIdx.x / LPR, col = threadIdx.x % LPR, r = group / share, sub = group % share;
-    const size_t step = (size_t)p.kv_heads * ROWS, at = ((size_t)t.base * p.kv_heads + kvh) * ROWS + r0 + min(r, rows - 1);
-    float m = -INFINITY, l = 0.f;
-    for (int s = col; s < t.splits; s += LPR) m = fmaxf(m, a.part_ml[at + s * step].x);
+    const int group = threadIdx.x / LPR, col = threadIdx.x % LPR;
+    const size_t step = (size_t)p.kv_heads * ROWS;
+    const int first = per_block * (b % blocks), last = min(t.rows, first + per_block);
+    for (int r0 = first; r0 < last; r0 += 16) {
+        const int rows = min(last - r0, 16);
+        int share = 1;  // groups of a row
+        while (2 * share * rows <= NG) share *= 2;
+        const int r = group / share, sub = group % share;
+        const size_t at = ((size_t)t.base * p.kv_heads + kvh) * ROWS + r0 + min(r, rows - 1);
+        float m = -INFINITY, l = 0.f;
+        for (int s = col; s < t.splits; s += LPR) m = fmaxf(m, a.part_ml[at + s * step].x);
 #pragma unroll
-    for (int d = 1; d < LPR; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int d = 1; d < LPR; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = sub; s < t.splits; s += share) {
-        const float2 ml = a.part_ml[at + s * step];
-        const float4 v = *reinterpret_cast<const float4*>(a.part + (at + s * step) * HD + 4 * col);
-        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // (no key seen: zeros)
-        l = fmaf(ml.y, f, l);
-        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+        for (int s = sub; s < t.splits; s += share) {
+            const float2 ml = a.part_ml[at + s * step];
+            const float4 v = *reinterpret_cast<const float4*>(a.part + (at + s * step) * HD + 4 * col);
+            const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);  // (no key seen: zeros)
+            l = fmaf(ml.y, f, l);
+            o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+        }
+        if (share > 1) {
+            if (r0 > first) __syncthreads();  // (the rows before have been read)
+            *reinterpret_cast<float4*>(&s_o[group][4 * col]) = o;
+            if (col == 0) s_l[group] = l;
+            __syncthreads();
+        }
+        if (sub != 0 || r >= rows) continue;
+        for (int k = 1; k < share; k++) {
+            const float4 v = *reinterpret_cast<const float4*>(&s_o[group + k][4 * col]);
+            o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+            l += s_l[group + k];
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int row = t.r0 + r0 + r, tok = row / p.group, head = kvh * p.group + row - tok * p.group;
+        store4((QT*)p.out + ((size_t)(t.first + tok) * p.heads + head) * HD + 4 * col, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
-    *reinterpret_cast<float4*>(&s_o[group][4 * col]) = o;
-    if (col == 0) s_l[group] = l;
-    __syncthreads();
-    if (sub != 0 || r >= rows) return;
-    for (int k = 1; k < share; k++) {
-        const float4 v = *reinterpret_cast<const float4*>(&s_o[group + k][4 * col]);
-        o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-        l += s_l[group + k];
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int row = t.r0 + r0 + r, tok = row / p.group, head = kvh * p.group + row - tok * p.group;
-    store4((QT*)p.out + ((size_t)(t.first + tok) * p.heads + head) * HD + 4 * col, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 template <int HD, typename QT>
 __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(16))) float s_o[512 / (HD / 4)][HD];
     __shared__ float s_l[512 / (HD / 4)];
-    const int kvh = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads, tiles = p.tile.target ? 8 * p.tile.tiles : 0;
+    const int kvh = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads;
+    const int tiles = p.tile.target ? 128 / p.merge_rows * p.tile.tiles : 0;
     if (b < tiles) merge_block<HD, QT, 128>(p, b, kvh, s_o, s_l);
     else merge_block<HD, QT, 16>(p, b - tiles, kvh, s_o, s_l);
 }
@@ -1450,7 +1460,7 @@ int launch_plan(const ar_pages* pages, const Plan& a, PagedParams p, char* work,
     else if (!p.few.tasks) hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 2>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 3>), grid, block, 0, st, p);
     AR_LAUNCH_CHECK();
-    const int merges = (p.tile.target ? 8 * p.tile.tiles : 0) + (p.few.target ? p.few.tiles : 0);
+    const int merges = (p.tile.target ? 128 / p.merge_rows * p.tile.tiles : 0) + (p.few.target ? p.few.tiles : 0);
     if (merges) {
         hipLaunchKernelGGL((paged_merge_kernel<HD, QT>), dim3((unsigned)merges * p.kv_heads), dim3(512), 0, st, p);
         AR_LAUNCH_CHECK();
@@ -1518,6 +1528,7 @@ extern "C" int ar_hip_attention_paged(ar_hip_ctx* ctx, const ar_pages* pages, in
     p.kv_heads = pages->kv_heads; p.group = heads / pages->kv_heads; p.seqs = pages->seqs;
     p.max_pages = pages->max_pages; p.pages = pages->pages; p.shift = page_shift_of(pages); p.n = chunks->n;
     p.rows = chunks->rows; p.few_rows = a.few_rows;
+    p.merge_rows = 8LL * a.tile.tiles * p.kv_heads > 4LL * ctx->num_cus ? 32 : 16;
     p.scale = (float)(1.4426950408889634 / std::sqrt((double)hd));
     char* const w = (char*)work;
     if (hd == 128)

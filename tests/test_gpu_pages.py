@@ -417,6 +417,22 @@ def test_attention_of_many_chunks(ctx, act, dtype, case):
     pool.free()
 
 
+def test_merging_blocks_of_two_row_groups_repeat(ctx):
+    """Enough tiles that a merging block takes two groups of rows, whose splits are shared (head size 64): the same bits
+    every time, and right."""
+    r = _rng(107)
+    n = 16
+    at, counts = [900 + 37 * i for i in range(n)], [64] * n
+    pool = Pool(ctx, r, "bf16", 1, 8, 64, 64, [a + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), 32, 64))
+    first = _attend(ctx, pool, 0, at, counts, q, "bf16", 32)
+    for _ in range(5):
+        np.testing.assert_array_equal(_attend(ctx, pool, 0, at, counts, q, "bf16", 32), first)
+    for i in (0, 7, 15):
+        _check_attention(first[64 * i:64 * i + 64], pool, 0, at[i:i + 1], [64], q[64 * i:64 * i + 64], "bf16", 32, seq=[i])
+    pool.free()
+
+
 @pytest.mark.parametrize("heads,kv,hd", [(96, 96, 64), (40, 40, 128), (300, 3, 64)])
 @pytest.mark.parametrize("counts", [[1, 1], [33, 1]])
 def test_attention_of_many_heads(ctx, heads, kv, hd, counts):
