@@ -321,19 +321,20 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         }
         keys = __int_as_float(lane_value(__float_as_int(wave_sum_lane63(keys)), 63));
         // (a little more than the even share, for the sum's roundings)
-        float share = fmaxf(kLeast<ROWS>, ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)));
+        const float share = fmaxf(kLeast<ROWS>, ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)));
+        const double inv = 1. / ((double)share * kUnit<ROWS>);
+        int per = (int)fminf(share, 1 << 24);  // (no chunk has more units)
         // That many units in a split are surely few enough tasks, with one more a tile.  Few rows, where the lanes hold
         // the units of all tiles: the fewest units whose tasks are all resident at once (16 sequences of 8,192 rows: 78 us
         // instead of 82, 40 of 2,000: 59 instead of 68).
         if (ROWS == 16 && p.n <= 64 && __ballot(n > 1) == 0) {
-            const float most = (float)min(p.few.blocks, p.few.tasks), u = (float)c.units, top = share;
-            for (share = fmaxf(kLeast<ROWS>, ceilf(keys / (most * kUnit<ROWS>)) - 1.f); share < top; share += 1.f) {
-                const float tasks = n == 0 ? 0.f : fmaxf(1.f, ceilf(u / share));
-                if (__int_as_float(lane_value(__float_as_int(wave_sum_lane63(tasks)), 63)) <= most) break;
-            }
+            const int most = min(p.few.blocks, p.few.tasks);
+            const float least = fmaxf(kLeast<ROWS>, ceilf(keys / ((float)most * kUnit<ROWS>)) - 1.f);
+            per = fewest_units((int)fminf(least, (float)per), per, [&](int units) {
+                const int tasks = n == 0 ? 0 : max(1, (c.units + units - 1) / units);
+                return lane_value(wave_scan(tasks), 63) <= most;
+            });
         }
-        const double inv = 1. / ((double)share * kUnit<ROWS>);
-        const int per = (int)fminf(share, 1 << 24);  // (no chunk has more units)
         int tasks = 0, tiles = 0;  // before these 64 chunks
         bool found = false;
         for (int i0 = 0; i0 < p.n && !found; i0 += 64) {

@@ -65,6 +65,18 @@ AR_HD int chunk_search(int n, int ways, F below) {
     return lo;
 }
 
+// Units of a split: the fewest in lo .. hi whose tasks `fits` accepts, or hi, where none below it is accepted.  `fits` is
+// monotone (more units in a split, fewer tasks).  At most log2(hi - lo) + 1 questions, whatever the answers are.
+template <typename F>
+AR_HD int fewest_units(int lo, int hi, F fits) {
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (fits(mid)) hi = mid;
+        else lo = mid + 1;
+    }
+    return hi;
+}
+
 // The chunk that holds row `row`, or -1.
 AR_HD int chunk_of_row(const int32_t* start, int n, int rows, int row) {
     if (row < 0 || row >= rows) return -1;

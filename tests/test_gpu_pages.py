@@ -417,6 +417,29 @@ def test_attention_of_many_chunks(ctx, act, dtype, case):
     pool.free()
 
 
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("case", ["long-among-short", "more-than-resident"])
+def test_attention_of_uneven_batches(ctx, act, dtype, case):
+    """Few-row chunks that fill one resident set of blocks: one long context among short ones, and (beside a chunk of
+    many rows) more chunks than there are blocks, for which no length of a split has all tasks resident."""
+    r = _rng(131)
+    if case == "long-among-short":
+        KV, G, counts = 8, 1, [1] * (31 if dtype == "f32" else 63)
+        at = r.integers(0, 200, len(counts)).tolist()
+        at[17] = 20000
+    else:
+        KV, G, counts = 32, 1, [1] * 40 + [1500]
+        at = r.integers(0, 700, len(counts)).tolist()
+        at[-1] = 30
+    pool = Pool(ctx, r, dtype, 1, KV, 64, 64, [a + c for a, c in zip(at, counts)])
+    q = r.standard_normal((sum(counts), KV * G, 64))
+    got = _attend(ctx, pool, 0, at, counts, q, act, KV * G)
+    starts, pick = _starts(counts), [0, 1, 17, len(counts) - 2, len(counts) - 1]
+    rows = np.concatenate([np.arange(starts[i], starts[i + 1]) for i in pick])
+    _check_attention(got[rows], pool, 0, [at[i] for i in pick], [counts[i] for i in pick], q[rows], act, KV * G, seq=pick)
+    pool.free()
+
+
 def test_merging_blocks_of_two_row_groups_repeat(ctx):
     """Enough tiles that a merging block takes two groups of rows, whose splits are shared (head size 64): the same bits
     every time, and right."""

@@ -25,6 +25,18 @@ def test_index_arithmetic_under_sanitizers(tmp_path):
     assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
 
 
+def test_tasks_of_attention_under_sanitizers(tmp_path):
+    """How attention cuts its keys: the fewest units of a split are found in some 25 questions at any accepted size."""
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    exe = str(tmp_path / "page_tasks")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-o",
+                    exe, os.path.join(ROOT, "tests", "sanitize", "page_tasks_main.cpp")], check=True)
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0:verify_asan_link_order=0")
+    r = subprocess.run([exe], capture_output=True, text=True, env=env, timeout=120)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
+
+
 def _pages(**over):
     f = dict(k=A, v=2 * A, table=A, rows=A, refs=A, dtype=hw.DTYPE_F32, layers=2, pages=8, kv_heads=2, page_rows=16,
              head_dim=64, seqs=3, max_pages=4)
