@@ -27,6 +27,7 @@
 #include <cmath>
 
 #include "page_common.h"
+#include "page_tasks.h"
 
 namespace {
 
@@ -209,30 +210,7 @@ struct Shape {
     static constexpr float BIAS = F16 ? 6.f : 0.f;  // weights scaled by 2^6 in fp16, and kSlack more: their small ones keep bits
 };
 
-// ---- what a block works on --------------------------------------------------------------------------------------
-// Tasks are the tiles of ROWS packed rows of every chunk.  Where there are enough of them to fill the GPU, a tile is a task
-// (target 0): the block's slot is searched among the chunks, 64 at a time.  Otherwise every block adds up what all
-// chunks' tiles see, so that splits of `per` units of kUnit<ROWS> keys make about `target` tasks of equal length whatever
-// the lengths of the sequences are, and finds its task in their order.  In a chunk of several tiles, tile j's tasks begin
-// at floor(S(j) / L) + j, with L keys in a split and S(j) the keys that the tiles before j see, from above and in closed
-// form: at least as many as its splits, and found without a sum over tiles; those past its splits are empty.
-template <int ROWS>
-constexpr int kUnit = ROWS == 16 ? 128 : 64;  // a round of the few-row kernel's wavefronts; the tile kernel's largest key tile
-
-// Units of a split, at least.  (One token over 4,096 rows in splits of one unit: 17.0 us, of two 14.1; tiles over few keys
-// want all the blocks they can get: 509 tokens over 609 rows 33.5 us, with two units 36.7.)
-template <int ROWS>
-constexpr float kLeast = ROWS == 16 ? 2.f : 1.f;
-
-struct Task {
-    int seq, first, count;  // chunk
-    int at;                 // cache row of its first token
-    int r0, rows;           // packed rows: first, and how many there are
-    int units;              // key units its chunk's last row sees
-    int per, splits, split; // units of a split, splits, and which
-    int base;               // the tile's first task
-};
-
+// ---- what a block works on (page_tasks.h) -----------------------------------------------------------------------
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // The table is read with scalar loads: nothing writes it while these kernels run.
 typedef const __attribute__((address_space(4))) int* TableRow;
@@ -247,32 +225,7 @@ __device__ __forceinline__ int chunk_tiles(const PagedParams& p, int i, Task* t)
     // (all loads at once)
     const int a = p.start ? p.start[j] : j, b = p.start ? p.start[j + 1] : j + 1;
     const int at = p.at[j], seq = p.seq ? p.seq[j] : j;
-    t->first = a;
-    t->count = i < p.n && a >= 0 && b > a && b <= p.rows ? b - a : 0;
-    t->seq = seq;
-    t->at = at;
-    const int cap = p.max_pages << p.shift;  // (at most 2^30)
-    const int end = at < 0 || seq < 0 || seq >= p.seqs ? 0 : at >= cap ? cap : min(at + t->count, cap);
-    t->units = (end + kUnit<ROWS> - 1) / kUnit<ROWS>;
-    const int packed = t->count * p.group;  // (at most 2^30)
-    if (t->count == 0 || (ROWS == 16 ? packed > p.few_rows : packed <= p.few_rows)) return 0;
-    return (packed + ROWS - 1) / ROWS;
-}
-
-// Keys that tile j of the chunk sees; S(j) above; first task of tile j.
-template <int ROWS>
-__device__ __forceinline__ int tile_end(const PagedParams& p, const Task& c, int j) {
-    const int cap = p.max_pages << p.shift, packed = c.count * p.group;
-    return c.units == 0 ? 0 : c.at >= cap ? cap : min(c.at + (min((j + 1) * ROWS, packed) - 1) / p.group + 1, cap);
-}
-template <int ROWS>
-__device__ __forceinline__ double keys_before(const PagedParams& p, const Task& c, int j) {
-    const double at = min(c.at, p.max_pages << p.shift) + 1;
-    return c.units == 0 ? 0. : j * at + 0.5 * ROWS * j * (j + 1.) / p.group;
-}
-template <int ROWS>
-__device__ __forceinline__ int first_task(const PagedParams& p, const Task& c, int j, double inv) {
-    return (int)(keys_before<ROWS>(p, c, j) * inv) + j;
+    return tiles_of_chunk<ROWS>(p, a, i < p.n ? b : a, at, seq, t);
 }
 
 // Sum over the lanes up to and with this one (row shifts, then row broadcasts).
@@ -313,33 +266,30 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
         // (of up to 64 chunks each lane keeps its own)
         Task c;
         int n = chunk_tiles<ROWS>(p, lane, &c);
-        float keys = n == 1 ? (float)c.units * kUnit<ROWS> : (float)keys_before<ROWS>(p, c, n);
+        float keys = keys_of_chunk<ROWS>(p, c, n);
         for (int i = lane + 64; i < p.n; i += 64) {
             Task d;
             const int k = chunk_tiles<ROWS>(p, i, &d);
-            keys += k == 1 ? (float)d.units * kUnit<ROWS> : (float)keys_before<ROWS>(p, d, k);
+            keys += keys_of_chunk<ROWS>(p, d, k);
         }
         keys = __int_as_float(lane_value(__float_as_int(wave_sum_lane63(keys)), 63));
-        // (a little more than the even share, for the sum's roundings)
-        const float share = fmaxf(kLeast<ROWS>, ceilf(keys * 1.0001f / ((float)target * kUnit<ROWS>)));
+        const float share = even_share<ROWS>(keys, target);
         const double inv = 1. / ((double)share * kUnit<ROWS>);
-        int per = (int)fminf(share, 1 << 24);  // (no chunk has more units)
+        int per = (int)fminf(share, kMostUnits);
         // That many units in a split are surely few enough tasks, with one more a tile.  Few rows, where the lanes hold
         // the units of all tiles: the fewest units whose tasks are all resident at once (16 sequences of 8,192 rows: 78 us
         // instead of 82, 40 of 2,000: 59 instead of 68).
         if (ROWS == 16 && p.n <= 64 && __ballot(n > 1) == 0) {
             const int most = min(p.few.blocks, p.few.tasks);
-            const float least = fmaxf(kLeast<ROWS>, ceilf(keys / ((float)most * kUnit<ROWS>)) - 1.f);
-            per = fewest_units((int)fminf(least, (float)per), per, [&](int units) {
-                const int tasks = n == 0 ? 0 : max(1, (c.units + units - 1) / units);
-                return lane_value(wave_scan(tasks), 63) <= most;
+            per = fewest_units(least_share<ROWS>(keys, most, per), per, [&](int units) {
+                return lane_value(wave_scan(n == 0 ? 0 : splits_of(c.units, units)), 63) <= most;
             });
         }
         int tasks = 0, tiles = 0;  // before these 64 chunks
         bool found = false;
         for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
             if (i0) n = chunk_tiles<ROWS>(p, i0 + lane, &c);
-            const int mine = n == 0 ? 0 : n == 1 ? max(1, (c.units + per - 1) / per) : first_task<ROWS>(p, c, n, inv);
+            const int mine = tasks_of_chunk<ROWS>(p, c, n, per, inv);
             const int a = wave_scan(mine), b = wave_scan(n);  // with this lane's chunk
             const unsigned long long m = __ballot((MERGE ? tiles + b : tasks + a) > index);
             if (m) {
@@ -351,19 +301,9 @@ __device__ __forceinline__ bool find_task(const PagedParams& p, int index, Task*
                 t->units = lane_value(c.units, l);
                 const int all = lane_value(n, l), a0 = tasks + lane_value(a, l) - lane_value(mine, l), b0 = tiles + lane_value(b, l) - all;
                 const int q = index - (MERGE ? b0 : a0);
-                if (MERGE || all == 1) {
-                    tile = MERGE ? q : 0;
-                } else {
-                    int hi = all - 1;  // the last tile whose tasks begin at q or before
-                    while (tile < hi) {
-                        const int mid = tile + (hi - tile + 1) / 2;
-                        if (first_task<ROWS>(p, *t, mid, inv) <= q) tile = mid;
-                        else hi = mid - 1;
-                    }
-                }
-                const int begin = all == 1 ? 0 : first_task<ROWS>(p, *t, tile, inv);
-                const int units = (tile_end<ROWS>(p, *t, tile) + kUnit<ROWS> - 1) / kUnit<ROWS>;
-                t->splits = max(1, (units + per - 1) / per);
+                tile = MERGE ? q : tile_of_task<ROWS>(p, *t, all, q, inv);
+                const int begin = tile_begin<ROWS>(p, *t, all, tile, inv);
+                t->splits = tile_splits<ROWS>(p, *t, tile, per);
                 t->split = MERGE ? 0 : q - begin;
                 t->base = a0 + begin;
                 found = true;
@@ -1387,67 +1327,20 @@ __global__ __launch_bounds__(512) void paged_merge_kernel(PagedParams p) {
 
 // ---- host side ----------------------------------------------------------------------------------------------
 
-// A kernel's share of a call: its tiles at most, and how many tasks to cut their keys into (0: none; one more per tile
-// for its last split, and one for what rounding makes of where its tasks begin).
-struct Part {
-    int tiles = 0, target = 0, blocks = 0;  // (blocks: resident at once)
-    int tasks() const { return target ? std::max(target + tiles + 1, blocks) : tiles; }
-    size_t bytes(const ar_pages* p, int rows) const {
-        return target ? (size_t)tasks() * p->kv_heads * rows * ((size_t)p->head_dim * 4 + 8) : 0;
-    }
-};
-
-// The launches of a call.  The host knows the numbers of rows and of chunks, not which chunk has how many.  Up to 32
-// packed rows a chunk on average, all chunks go to the few-row kernel (16 sequences, 8 tokens, 4 heads a KV head, 22 rows
-// on average: 36 us, tiles 46; 16 tokens, 45 rows: 49 us, tiles 39).  One chunk of more rows goes to the tile kernel.
-// Otherwise one launch holds both kernels' blocks, and chunks of up to kFewRows rows are the few-row kernel's (decode
-// steps and a prompt together, fp16 and fp32: 143 and 290 us, all as tiles 162 and 338; kFewRows 64 instead of 16: 16
-// chunks of 16 tokens 53 us instead of 39 in bf16, 63 instead of 44 in fp32).
-struct Plan {
-    int few_rows = 0;  // packed rows up to which a chunk is the few-row kernel's
-    Part few, tile;
-};
-
-constexpr int kFewRows = 16, kMaxSplitChunks = 1024;
-
-// Tasks to cut the keys for: `per_cu` blocks a CU over all KV heads, the number that is resident at once, unless the tiles
-// alone are as many (1,024 tokens of three sequences, 537 tiles for 512 blocks: whole tiles 609 us, cut ones 632).
-void cut_keys(const ar_hip_ctx* ctx, const ar_pages* p, long long tiles, int n, int per_cu, int unit, Part* out) {
-    const long long blocks = (long long)per_cu * ctx->num_cus / p->kv_heads, cap = (long long)p->max_pages * p->page_rows;
-    if (tiles >= blocks || n > kMaxSplitChunks) return;
-    if (cap <= unit) return;  // (one split of any sequence)
-    // (a tile's last split is a task of its own, so that there may be `tiles` more; and no more than units)
-    const long long want = std::min(blocks - tiles, std::max<long long>(tiles, n) * ((cap + unit - 1) / unit));
-    out->target = (int)std::max(1LL, want);
-    out->blocks = (int)blocks;
+size_t part_bytes(const ar_pages* p, const Part& a, int rows) {
+    return a.target ? (size_t)a.tasks() * p->kv_heads * rows * ((size_t)p->head_dim * 4 + 8) : 0;
 }
 
 int plan_of(const ar_hip_ctx* ctx, const ar_pages* p, const ar_chunks* c, int heads, Plan* out) {
     const long long group = heads / p->kv_heads, packed = (long long)c->rows * group;
     AR_CHECK_ARG(packed <= 1 << 30 && (packed / 16 + c->n) * p->kv_heads < 1 << 23, "paged attention: %d rows of %d heads are too many",
                  c->rows, heads);
-    Plan a;
-    // (Few rows over fp32, which keep twice the bytes in flight: one block a CU, 46 us for 8 sequences of 4,000 rows, two
-    // 52; 16-bit caches: two, 82 us for 16 of 8,192, one 88.  Tiles: two, 46 us for the fp32 chunk, one 52.)
-    const int few_cu = p->dtype == AR_DTYPE_F32 ? 1 : 2, tile_cu = 2;
-    if (!c->start || packed <= 32LL * c->n) {
-        a.few_rows = 0x7fffffff;
-        a.few.tiles = (int)(c->start ? packed / 16 + c->n : c->n * ((group + 15) / 16));
-        cut_keys(ctx, p, std::max<long long>(c->n, packed / 16), c->n, few_cu, kUnit<16>, &a.few);
-    } else {
-        a.tile.tiles = (int)(packed / 128 + c->n);
-        cut_keys(ctx, p, packed / 128, c->n, tile_cu, kUnit<128>, &a.tile);
-        if (c->n > 1) {
-            a.few_rows = kFewRows;
-            cut_keys(ctx, p, 0, c->n, few_cu, kUnit<16>, &a.few);
-            a.few.tiles = (int)(a.few.target ? std::min(packed / 16 + c->n, kFewRows / 16LL * c->n) : packed / 16 + c->n);
-        }
-    }
-    *out = a;
+    *out = plan_tasks(ctx->num_cus, p->kv_heads, p->dtype == AR_DTYPE_F32, (long long)p->max_pages * p->page_rows, c->start != nullptr,
+                      c->n, c->rows, (int)group);
     return AR_HIP_OK;
 }
 
-size_t plan_bytes(const ar_pages* p, const Plan& a) { return std::max<size_t>(16, a.few.bytes(p, 16) + a.tile.bytes(p, 128)); }
+size_t plan_bytes(const ar_pages* p, const Plan& a) { return std::max<size_t>(16, part_bytes(p, a.few, 16) + part_bytes(p, a.tile, 128)); }
 
 template <int HD, typename QT, typename KT>
 int launch_plan(const ar_pages* pages, const Plan& a, PagedParams p, char* work, hipStream_t st) {
@@ -1455,7 +1348,7 @@ int launch_plan(const ar_pages* pages, const Plan& a, PagedParams p, char* work,
         return PartArgs{x.tiles, x.tasks(), x.target, x.blocks, (float*)at, (float2*)(at + (size_t)x.tasks() * p.kv_heads * rows * HD * 4)};
     };
     p.few = part(a.few, 16, work);
-    p.tile = part(a.tile, 128, work + a.few.bytes(pages, 16));
+    p.tile = part(a.tile, 128, work + part_bytes(pages, a.few, 16));
     const dim3 grid((unsigned)(p.few.tasks + p.tile.tasks) * p.kv_heads), block(kThreads);
     if (!p.tile.tasks) hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 1>), grid, block, 0, st, p);
     else if (!p.few.tasks) hipLaunchKernelGGL((paged_attention_kernel<HD, QT, KT, 2>), grid, block, 0, st, p);

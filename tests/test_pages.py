@@ -26,7 +26,8 @@ def test_index_arithmetic_under_sanitizers(tmp_path):
 
 
 def test_tasks_of_attention_under_sanitizers(tmp_path):
-    """How attention cuts its keys: the fewest units of a split are found in some 25 questions at any accepted size."""
+    """How attention cuts its keys: every split of every tile has a task of its own below the number of tasks, and the
+    fewest units of a split are found in some 25 questions at any accepted size."""
     if shutil.which("g++") is None:
         pytest.skip("g++ not available")
     exe = str(tmp_path / "page_tasks")
