@@ -46,7 +46,9 @@ typedef struct ar_pages {
 /* The new rows of a call, by sequence: chunk i is the rows start[i] .. start[i+1]-1 of the call's row arrays, and
  * they are the rows at[i], at[i]+1, ... of sequence seq[i].  Rows from start[n] on belong to no chunk: they are
  * neither read nor written.  A chunk of an unknown sequence or with a negative at is not in the cache: its rows are
- * dropped when written and see nothing.  A row past the table's last column is dropped, too. */
+ * dropped when written and see nothing.  A row past the table's last column is dropped, too.  A chunk that passes the
+ * call's rows is empty; where starts descend it is not defined which chunks are (no access leaves the arrays, and rows
+ * are left as they were or computed). */
 typedef struct ar_chunks {
     const int32_t *seq;   /* device [n], or null: sequences 0 .. n-1 */
     const int32_t *start; /* device [n+1], not decreasing, from 0; or null: one row each */

@@ -275,6 +275,39 @@ def test_attention_with_chunk_starts_of_anything_stays_inside(ctx):
     pool.free()
 
 
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("heads", [2, 64])
+@pytest.mark.parametrize("starts,sure", [
+    ([0, 10, 25, 90, 95], [0, 1]), ([0, 7, 7, 40, 41], [0, 1, 2]), ([41, 50, 60, 70, 80], []), ([5, 5, 5, 5, 5], []),
+    ([3, 20, 20, 33, 40], [0, 2, 3]), ([0, 40, 0, 40, 0], None), ([-7, 3, 20, 2 ** 31 - 1, 9], None)])
+def test_attention_leaves_rows_of_no_chunk(ctx, act, dtype, heads, starts, sure):
+    """Starts in order whose chunks pass the rows: those chunks are empty, the others are right and nothing else is
+    written.  Starts that descend (None): a row is as it was, or finite (zero or an average of values of its pool)."""
+    r = _rng(139)
+    pool = Pool(ctx, r, dtype, 1, 2, 64, 16, [60, 60, 60, 60])
+    q, at = r.standard_normal((40, heads, 64)), [20, 3, 0, 20]
+    host = ref.to_bits(q, act)
+    mark = np.full(host.shape, 0x4321 if act == "bf16" else 7.25, ref.STORED[act])
+    qd, od, a, st = ctx.to_device(host), ctx.to_device(mark), _i32(ctx, at), _i32(ctx, starts)
+    pool.cache.attention(0, pg.Chunks(4, 40, at=a, start=st), qd, od, heads, CODE[act])
+    ctx.synchronize()
+    got = od.download(host.dtype, host.size).reshape(host.shape)
+    if sure is None:
+        top = np.abs(ref.values(pool.v)).max() * 1.01
+        assert ((got == mark) | (np.abs(ref.values(got)) <= top)).all()
+    else:
+        left = np.ones(40, bool)
+        for i in sure:
+            x, y = starts[i], starts[i + 1]
+            left[x:y] = False
+            if y > x:
+                _check_attention(ref.values(got[x:y]), pool, 0, at[i:i + 1], [y - x], q[x:y], act, heads, seq=[i])
+        np.testing.assert_array_equal(got[left], mark[left])
+    for b in (qd, od, a, st):
+        b.free()
+    pool.free()
+
+
 def test_attention_repeats_bit_for_bit(ctx):
     r = _rng(29)
     pool = Pool(ctx, r, "f16", 1, 2, 128, 64, [5000, 700])
