@@ -269,6 +269,8 @@ class HipContext:
         check(lib().ar_hip_init(-1 if device is None else device, ctypes.byref(h)))
         self.handle = h.value
         self.device = device
+        # the device's number also where the environment chose it
+        self.index = device if device is not None and device >= 0 else int(os.environ.get("AR_HIP_DEVICE") or 0)
 
     def close(self):
         if self.handle:

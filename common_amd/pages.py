@@ -146,8 +146,17 @@ class PagedCache:
         check(lib().ar_hip_pages_compact(self.ctx.handle, self.ref, _ptr(live), w.ptr, w.nbytes))
 
     def copy(self, to: "PagedCache", src, dst, n: int):
-        """Page src[i] of this pool becomes page dst[i] of `to`, in every layer (ar_hip_pages_copy)."""
+        """Page src[i] of this pool becomes page dst[i] of `to`, in every layer (ar_hip_pages_copy).  A cache of another
+        context on the same device: the host waits for that context's queued work before the copy and for the copy
+        after it, so that it has its place in both streams; on another device: refused."""
+        other = to.ctx is not self.ctx
+        if other:
+            if to.ctx.index != self.ctx.index:
+                raise ValueError(f"pages of device {self.ctx.index} cannot be copied to device {to.ctx.index}")
+            to.ctx.synchronize()
         check(lib().ar_hip_pages_copy(self.ctx.handle, self.ref, to.ref, _ptr(src), _ptr(dst), n))
+        if other:
+            self.ctx.synchronize()
 
     def write(self, layer: int, chunks: Chunks, q, k, v, q_out, heads: int, rotary: Rotary, act_dtype: int = DTYPE_F32,
               q_stride: int = 0, kv_stride: int = 0, q_norm=None, k_norm=None, eps: float = 1e-6, qk_norm_mode: int = 0):

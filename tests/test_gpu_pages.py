@@ -927,6 +927,31 @@ def test_copy_between_pools(ctx):
     b.free()
 
 
+def test_copy_to_a_cache_of_another_context(ctx):
+    """The other context's queued work on the target pages comes before the copy, its later work after it."""
+    r = _rng(151)
+    with hw.HipContext(0) as other:
+        a, b, c = (Pool(x, r, "f32", 4, 8, 128, 64, [64 * 60], spare=4) for x in (ctx, other, other))
+        pages = len(a.refs)
+        all_pages = [_i32(ctx, r.permutation(pages)) for _ in range(2)]
+        assert ctx.index == other.index == 0
+        for _ in range(3):
+            for k in range(4):  # (each of 67 MB of keys and as much of values)
+                c.cache.copy(b.cache, all_pages[0], all_pages[0], pages)
+            a.cache.copy(b.cache, all_pages[1], all_pages[1], pages)
+            b.cache.copy(c.cache, all_pages[0], all_pages[0], pages)
+            other.synchronize()
+            for x, y in ((b, a), (c, a)):
+                np.testing.assert_array_equal(x.down("k"), a.k)
+                np.testing.assert_array_equal(x.down("v"), a.v)
+            c.set("k", c.k)
+            c.set("v", c.v)
+        for x in all_pages:
+            x.free()
+        for x in (a, b, c):
+            x.free()
+
+
 def test_copy_within_a_pool(ctx):
     pool = Pool(ctx, _rng(9), "f32", 2, 1, 64, 16, [160], spare=2)
     src, dst = [0, 1, 2, 3, 3, 6], [7, 0, 8, 8, 9, 6]  # target 0 is a source, target 8 is named twice, 6 is its own

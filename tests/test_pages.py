@@ -256,3 +256,35 @@ def test_calls_after_close_are_refused():
                  lambda: cache.compact(), lambda: cache.copy(cache, at, at, 1)):
         with pytest.raises(Exception, match="no keys"):
             call()
+
+
+def test_copy_to_a_cache_of_another_context(monkeypatch):
+    """On one device it is ordered with both contexts' work; on another device it is refused before the library."""
+    class Buf:
+        ptr = A
+
+    class Ctx:
+        def __init__(self, name, index):
+            self.name, self.index, self.handle = name, index, A
+
+        def synchronize(self):
+            done.append(self.name)
+
+    class Lib:
+        def ar_hip_pages_copy(self, *args):
+            done.append("copy")
+            return hw.AR_HIP_OK
+
+    done = []
+    monkeypatch.setattr(pg, "lib", Lib)
+    a, b, c = (pg.PagedCache(x, 1, 4, 1, 64, 1, 1, k=Buf, v=Buf, table=Buf, rows=Buf, refs=Buf)
+               for x in (Ctx("a", 0), Ctx("b", 0), Ctx("c", 1)))
+    a.copy(a, Buf, Buf, 1)
+    assert done == ["copy"]
+    done.clear()
+    a.copy(b, Buf, Buf, 1)
+    assert done == ["b", "copy", "a"]
+    done.clear()
+    with pytest.raises(ValueError, match="device"):
+        a.copy(c, Buf, Buf, 1)
+    assert not done
