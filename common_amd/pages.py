@@ -23,6 +23,7 @@ import numpy as np
 from .hardware import DTYPE_BF16, DTYPE_F16, DTYPE_F32, HipContext, check, lib
 
 ROPE_SECTIONS, ROPE_INTERLEAVED = 0, 1
+KEPT_SIZES = 64  # work sizes that a cache keeps
 ELEM_BYTES = {DTYPE_F32: 4, DTYPE_BF16: 2, DTYPE_F16: 2}
 
 
@@ -119,12 +120,21 @@ class PagedCache:
             self._work.append(self.ctx.allocate(max(need, 2 * self._work[-1].nbytes if self._work else 0)))
         return self._work[-1]
 
-    def _table_scratch(self, n):
-        if n not in self._need:
+    def _work_bytes(self, key, ask):
+        """Work bytes of a kind of call, by `ask(bytes)` where they are not known.  Some are kept, not all that
+        there ever were: a server's row counts differ from step to step."""
+        need = self._need.get(key)
+        if need is None:
             b = ctypes.c_size_t()
-            check(lib().ar_hip_pages_work(self.ref, n, ctypes.byref(b)))
-            self._need[n] = b.value
-        return self._scratch(self._need[n])
+            check(ask(ctypes.byref(b)))
+            need = b.value
+            if len(self._need) >= KEPT_SIZES:
+                self._need.clear()
+            self._need[key] = need
+        return need
+
+    def _table_scratch(self, n):
+        return self._scratch(self._work_bytes(n, lambda b: lib().ar_hip_pages_work(self.ref, n, b)))
 
     def grow(self, chunks: Chunks, missing=None):
         """Room for the chunks' rows at their sequences' ends; fills chunks.at (ar_hip_pages_grow)."""
@@ -169,11 +179,8 @@ class PagedCache:
 
     def attention(self, layer: int, chunks: Chunks, q, out, heads: int, act_dtype: int = DTYPE_F32):
         """Causal attention of the chunks' rows over their sequences' pages (ar_hip_attention_paged)."""
-        key = (chunks.n, chunks.rows, chunks.start is None, heads)
-        if key not in self._need:
-            b = ctypes.c_size_t()
-            check(lib().ar_hip_attention_paged_work(self.ctx.handle, self.ref, chunks.ref, heads, ctypes.byref(b)))
-            self._need[key] = b.value
-        w = self._scratch(self._need[key])
+        w = self._scratch(self._work_bytes(
+            (chunks.n, chunks.rows, chunks.start is None, heads),
+            lambda b: lib().ar_hip_attention_paged_work(self.ctx.handle, self.ref, chunks.ref, heads, b)))
         check(lib().ar_hip_attention_paged(self.ctx.handle, self.ref, layer, chunks.ref, _ptr(q), act_dtype, heads,
                                            _ptr(out), w.ptr, w.nbytes))

@@ -288,3 +288,37 @@ def test_copy_to_a_cache_of_another_context(monkeypatch):
     with pytest.raises(ValueError, match="device"):
         a.copy(c, Buf, Buf, 1)
     assert not done
+
+
+def test_a_cache_keeps_few_work_sizes(monkeypatch):
+    """A server's row counts differ in every step: what the cache keeps of them has an end, and sizes stay right."""
+    class Buf:
+        ptr, nbytes = A, 1 << 40
+
+    class Ctx:
+        handle = A
+
+    class Lib:
+        def ar_hip_attention_paged_work(self, ctx, pages, chunks, heads, out):
+            asked.append(chunks._obj.rows)
+            out._obj.value = 1000 + chunks._obj.rows
+            return hw.AR_HIP_OK
+
+        def ar_hip_pages_work(self, pages, n, out):
+            out._obj.value = 10 + n
+            return hw.AR_HIP_OK
+
+        def ar_hip_attention_paged(self, *args):
+            return hw.AR_HIP_OK
+
+    asked, needed = [], []
+    monkeypatch.setattr(pg, "lib", Lib)
+    cache = pg.PagedCache(Ctx(), 1, 4, 1, 64, 1, 1, k=Buf, v=Buf, table=Buf, rows=Buf, refs=Buf)
+    cache._work.append(Buf)
+    monkeypatch.setattr(cache, "_scratch", lambda need: needed.append(need) or Buf)
+    for rows in list(range(1, 500)) + [499, 1]:
+        cache.attention(0, pg.Chunks(1, rows, at=Buf, start=Buf), Buf, Buf, 1)
+        assert needed[-1] == 1000 + rows and len(cache._need) <= 64
+        cache._table_scratch(rows)
+        assert needed[-1] == 10 + rows and len(cache._need) <= 64
+    assert asked == list(range(1, 500)) + [1]
