@@ -93,10 +93,15 @@ class PagedCache:
             return buf
 
         pool = layers * pages * kv_heads * page_rows * head_size * ELEM_BYTES[dtype]
-        self.k, self.v = take(k, pool, None), take(v, pool, None)
-        self.table = take(table, seqs * max_pages * 4, -1)
-        self.rows = take(rows, seqs * 4, 0)
-        self.refs = take(refs, pages * 4, 0)
+        try:
+            self.k, self.v = take(k, pool, None), take(v, pool, None)
+            self.table = take(table, seqs * max_pages * 4, -1)
+            self.rows = take(rows, seqs * 4, 0)
+            self.refs = take(refs, pages * 4, 0)
+        except Exception:  # (out of memory: nothing of a cache that does not come to be stays)
+            for buf in self._own:
+                buf.free()
+            raise
         self.raw = ArPages(_ptr(self.k), _ptr(self.v), _ptr(self.table), _ptr(self.rows), _ptr(self.refs), dtype,
                            layers, pages, kv_heads, page_rows, head_size, seqs, max_pages)
         self.ref = ctypes.byref(self.raw)

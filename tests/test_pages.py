@@ -322,3 +322,31 @@ def test_a_cache_keeps_few_work_sizes(monkeypatch):
         cache._table_scratch(rows)
         assert needed[-1] == 10 + rows and len(cache._need) <= 64
     assert asked == list(range(1, 500)) + [1]
+
+
+@pytest.mark.parametrize("room", range(5))
+def test_a_cache_that_does_not_fit_leaves_nothing_behind(room):
+    """Whichever of its buffers cannot be had, those before it are given back."""
+    class Buf:
+        ptr, freed = A, False
+
+        def upload(self, a):
+            pass
+
+        def free(self):
+            self.freed = True
+
+    class Ctx:
+        def __init__(self):
+            self.made = []
+
+        def allocate(self, nbytes):
+            if len(self.made) == room:
+                raise hw.HardwareException(1, "out of memory")
+            self.made.append(Buf())
+            return self.made[-1]
+
+    ctx = Ctx()
+    with pytest.raises(hw.HardwareException, match="out of memory"):
+        pg.PagedCache(ctx, 1, 4, 1, 64, 2, 2)
+    assert len(ctx.made) == room and all(b.freed for b in ctx.made)
