@@ -432,6 +432,10 @@ def _handle(s):
         n = case["seqs"] // 3
         h["old"] = [SimpleNamespace(ptr=t.data_ptr()) for t in s["old"]]
         h["chunks"] = [pg.Chunks(n, sum(_contexts(case)[:n]), start=b["start"], at=b["at"], seq=o) for o in h["old"]]
+    # The inputs were made on torch's stream, and the context has its own: they are ready before its first call.  (A
+    # program reads results, or stops a clock, behind a synchronisation of the device or the context, as it would after
+    # any call of the context's; nothing else orders the two streams.)
+    torch.cuda.synchronize()
     s["handle"] = h
     return h
 
