@@ -1211,3 +1211,43 @@ def test_pointer_checks_cover_the_paged_calls():
     lines = p.stdout.split("\n")
     assert lines[0].startswith("checked") and int(lines[0].split()[1]) > 40, p.stdout
     assert lines[1:6] == ["refused True"] * 5, p.stdout
+
+
+TIMED = """
+import torch
+import perf.operators as cases
+
+def outputs(o):
+    return o if isinstance(o, dict) else {"out": o}
+
+listed = {c["name"]: c for c in cases.listed()}
+a = torch.ones(8192, 8192, device="cuda")
+for name in ("write-image-prompt", "copy-few", "turnover-6", "attention-chunk-f32"):
+    print(name, flush=True)
+    case = listed[name]
+    want = outputs(cases.run(cases.prepare(case, 5)))
+    torch.cuda.synchronize()
+    cases.own = True
+    cases.run(cases.prepare(case, 6))  # (the context is made)
+    torch.cuda.synchronize()
+    for _ in range(4):  # some 30 ms, ahead of the inputs
+        a @ a
+    got = outputs(cases.run(cases.prepare(case, 5)))
+    torch.cuda.synchronize()
+    cases.own = False
+    for key, w in want.items():
+        # half a step of 16-bit results on either side; fp32 sums: (64 u S + 32 u) W with S below 20 and W below 1
+        w, g = w.double(), got[key].double()
+        tol = {torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}.get(want[key].dtype, 0.0) * w.abs() + 1e-4
+        assert want[key].is_floating_point() or (w == g).all(), (name, key)
+        assert ((g - w).abs() <= tol).all(), (name, key, float((g - w).abs().max()))
+print("ok")
+"""
+
+
+def test_timed_cases_wait_for_their_inputs():
+    """The timed cases' inputs are made on torch's stream while the context has its own: the first call on new inputs
+    finds them whole, with work still queued on torch's stream when they are made."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", TIMED], cwd=root, capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and r.stdout.endswith("ok\n"), r.stdout + r.stderr
