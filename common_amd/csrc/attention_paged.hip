@@ -139,9 +139,10 @@ __device__ __forceinline__ floatx4 mac4f(unsigned a, float b, floatx4 c) {
 }
 __device__ __forceinline__ floatx4 mac4(unsigned a, unsigned b, floatx4 c) { return mac4f(a, __uint_as_float(b), c); }
 
-// Power of two that brings a row whose largest finite value is `top` into fp16's range, its largest to [2^14, 2^15);
-// at most 2^100, also for a row of zeros.
-__device__ __forceinline__ int fp16_shift(float top) { return min(141 - (int)(__float_as_uint(top) >> 23), 100); }
+// Power of two that brings a row whose largest finite value is `top` into fp16's range, its largest to [2^14, 2^15); at
+// most 2^122, also for a row of zeros (a row of values below 2^-108 to less, one below 2^-122 with fewer bits; and a
+// score's scale times its inverse is still a normal number).
+__device__ __forceinline__ int fp16_shift(float top) { return min(141 - (int)(__float_as_uint(top) >> 23), 122); }
 
 // maximum over the LANES (8 or 16) lanes that hold a row; of values >= 0, as their bits (which need no canonical form)
 template <int LANES>

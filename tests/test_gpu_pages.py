@@ -359,6 +359,22 @@ def test_rows_of_very_different_magnitudes(ctx, act, hd, at, counts):
     pool.free()
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("at,counts", [([700, 3], [1, 1]), ([300], [160]), ([5, 90, 0], [70, 1, 40])])
+def test_rows_of_tiny_values(ctx, act, hd, at, counts):
+    """fp32 rows near the smallest normal number (keys under queries that bring scores to ordinary size) keep their
+    bits."""
+    r = _rng(149)
+    pool = Pool(ctx, r, "f32", 1, 2, hd, 16, [a + c for a, c in zip(at, counts)])
+    pool.set("v", (pool.v * 2.0 ** -116).astype(np.float32))
+    pool.set("k", (pool.k * 2.0 ** -118).astype(np.float32))
+    q = 2.0 ** 118 * r.standard_normal((sum(counts), 4, hd))
+    got = _attend(ctx, pool, 0, at, counts, q, act, 4)
+    _check_attention(got, pool, 0, at, counts, q, act, 4)
+    pool.free()
+
+
 @pytest.mark.parametrize("act,dtype", [("bf16", "f32"), ("bf16", "bf16"), ("bf16", "f16")])
 def test_a_first_tile_of_scores_of_minus_infinity(ctx, act, dtype):
     """Visible keys whose scores are -inf have no weight, also where nothing else has been seen yet.  (bf16 queries: of
