@@ -149,11 +149,11 @@ inline void cut_keys(long long blocks, long long cap, long long tiles, int n, in
     out->blocks = (int)blocks;
 }
 
-// Of n chunks (`starts`: of any lengths, not one row each) with `rows` rows in all and `group` query heads a KV head, over
-// tables of `cap` rows of `kv_heads` KV heads, fp32 or not, on a GPU of `cus` CUs.
+// Of n chunks (`starts`: of any lengths, not one row each; the rows behind those are no work) with `rows` rows in all and
+// `group` query heads a KV head, over tables of `cap` rows of `kv_heads` KV heads, fp32 or not, on a GPU of `cus` CUs.
 inline Plan plan_tasks(int cus, int kv_heads, bool fp32, long long cap, bool starts, int n, int rows, int group) {
     Plan a;
-    const long long packed = (long long)rows * group;
+    const long long packed = (starts ? rows : n) * (long long)group;
     // (Few rows over fp32, which keep twice the bytes in flight: one block a CU, 46 us for 8 sequences of 4,000 rows, two
     // 52; 16-bit caches: two, 82 us for 16 of 8,192, one 88.  Tiles: two, 46 us for the fp32 chunk, one 52.)
     const long long few = (fp32 ? 1LL : 2LL) * cus / kv_heads, tile = 2LL * cus / kv_heads;

@@ -152,7 +152,21 @@ static void every_split_has_a_task() {
     CHECK(cut[0] > 5000 && cut[1] > 5000 && whole > 5000);
 }
 
+// Chunks of one row each in row arrays of a fixed size: the rows behind them change nothing.
+static void rows_behind_single_tokens() {
+    for (int t = 0; t < 2000; t++) {
+        const int cus = pick(1, 304), kv_heads = pick(1, 40), n = pick(1, 1100), group = pick(1, 40);
+        const long long cap = 1LL << pick(4, 30);
+        const bool fp32 = pick(0, 1);
+        const Plan a = plan_tasks(cus, kv_heads, fp32, cap, false, n, n, group);
+        const Plan b = plan_tasks(cus, kv_heads, fp32, cap, false, n, n + pick(1, 1 << 22), group);
+        CHECK(a.few_rows == b.few_rows && a.few.tiles == b.few.tiles && a.few.target == b.few.target && a.few.blocks == b.few.blocks);
+        CHECK(a.tile.tasks() == 0 && b.tile.tasks() == 0);
+    }
+}
+
 int main() {
+    rows_behind_single_tokens();
     every_split_has_a_task();
     fewest_units_of_a_split();
     printf("ok\n");

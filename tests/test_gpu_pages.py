@@ -489,6 +489,19 @@ def test_attention_of_uneven_batches(ctx, act, dtype, case):
     pool.free()
 
 
+@pytest.mark.parametrize("act,dtype", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+def test_single_tokens_in_longer_row_arrays(ctx, act, dtype):
+    """Row arrays of a fixed size: the rows behind the last chunk stay as they are and change no result."""
+    r = _rng(157)
+    pool = Pool(ctx, r, dtype, 1, 2, 64, 64, [3000, 40, 700])
+    at, q = [2999, 39, 5], r.standard_normal((3, 8, 64))
+    first = _attend(ctx, pool, 0, at, [1, 1, 1], q, act, 8, one_each=True, extra=0)
+    _check_attention(first, pool, 0, at, [1, 1, 1], q, act, 8)
+    for extra in (1, 61, 5000):
+        np.testing.assert_array_equal(_attend(ctx, pool, 0, at, [1, 1, 1], q, act, 8, one_each=True, extra=extra), first)
+    pool.free()
+
+
 def test_merging_blocks_of_two_row_groups_repeat(ctx):
     """Enough tiles that a merging block takes two groups of rows, whose splits are shared (head size 64): the same bits
     every time, and right."""
