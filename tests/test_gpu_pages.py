@@ -935,6 +935,37 @@ def test_compact(ctx, lengths, pages_spare):
     pool.free()
 
 
+@pytest.mark.parametrize("seed,P,spare,cols", [(1, 16, 3, 6), (2, 16, 12, 4), (3, 64, 40, 9), (4, 256, 6, 3)])
+def test_table_calls_in_any_order(ctx, seed, P, spare, cols):
+    """Sequences that come, share, grow, run out of pages, are cut back and moved: every call against the reference,
+    and the counts against the table."""
+    r = _rng(1000 + seed)
+    seqs = 7
+    pool = Pool(ctx, r, ["f16", "f32", "bf16", "f32"][seed - 1], 1, 1, 64, P, [P + 5, 2 * P, 3, 0], seqs=seqs, cols=cols, spare=spare)
+    t = _tables(pool)
+    for step in range(60):
+        kind = r.integers(0, 8)
+        some = r.permutation(seqs)[:r.integers(1, seqs + 1)].tolist()
+        if kind < 4:
+            counts = [int(r.choice([0, 1, 1, 2, P - 1, P, P + 1, 2 * P])) for _ in some]
+            if kind == 0:  # (one of them twice)
+                some, counts = some + some[:1], counts + [1]
+            _grow(ctx, pool, t, counts, some)
+        elif kind < 6:
+            keep = [int(r.choice([0, 1, P - 1, P, P + 1, 3 * P])) for _ in some] if r.integers(0, 3) else None
+            _trim(ctx, pool, t, some, keep)
+        elif kind == 6:
+            _fork(ctx, pool, t, r.integers(-1, seqs + 1, len(some)).tolist(), r.integers(0, seqs, len(some)).tolist())
+        else:
+            pool.cache.compact(None)
+            t.compact()
+            ctx.synchronize()
+        _same(pool, t)
+        held = np.bincount(t.table[t.table >= 0], minlength=len(t.refs))
+        np.testing.assert_array_equal(held, t.refs)
+    pool.free()
+
+
 def test_copy_between_pools(ctx):
     r = _rng(8)
     a = Pool(ctx, r, "f16", 3, 2, 128, 32, [320], spare=2)
