@@ -129,7 +129,9 @@ struct Part {
 // on average: 36 us, tiles 46; 16 tokens, 45 rows: 49 us, tiles 39).  One chunk of more rows goes to the tile kernel.
 // Otherwise one launch holds both kernels' blocks, and chunks of up to kFewRows rows are the few-row kernel's (decode
 // steps and a prompt together, fp16 and fp32: 143 and 290 us, all as tiles 162 and 338; kFewRows 64 instead of 16: 16
-// chunks of 16 tokens 53 us instead of 39 in bf16, 63 instead of 44 in fp32).
+// chunks of 16 tokens 53 us instead of 39 in bf16, 63 instead of 44 in fp32).  The average also sends one longer chunk
+// among many single tokens to the few-row kernel: 127 tokens over 1,500 rows and 512 over 1,512, 32 / 8 heads of 128, 194
+// us in bf16, the two apart 151 and 46.
 struct Plan {
     int few_rows = 0;  // packed rows up to which a chunk is the few-row kernel's
     Part few, tile;
@@ -139,7 +141,8 @@ constexpr int kFewRows = 16, kMaxSplitChunks = 1024;
 
 // Tasks to cut the keys for, of n chunks over tables of `cap` rows: `blocks`, the number that is resident at once, unless
 // the tiles alone are as many (1,024 tokens of three sequences, 537 tiles for 512 blocks: whole tiles 609 us, cut ones
-// 632).
+// 632).  Each tile takes one of them, so that a long context among nearly as many short ones is hardly cut: 31,999 rows
+// beside 62 (63) of 1,000 in fp16, 8 KV heads: 217 us (372), 79 by their bytes; beside 30: 52, its floor.
 inline void cut_keys(long long blocks, long long cap, long long tiles, int n, int unit, Part* out) {
     if (tiles >= blocks || n > kMaxSplitChunks) return;
     if (cap <= unit) return;  // (one split of any sequence)

@@ -132,8 +132,9 @@ int ar_hip_pages_write(ar_hip_ctx *ctx, const ar_pages *pages, int layer, const 
  * aligned; out may be q itself.  Rows that see nothing become 0.  What a hidden row holds (infinities, NaN) does not
  * reach the result; infinities and NaN that a row sees make it infinite or NaN.
  * Sums are in fp32, of weights up to 2^14: keys and values beyond 2^90 may overflow them.  With fp32 activations the products
- * keep 22 bits or more: relative to each factor over 16-bit caches, to the largest value of its row of the cache over
- * fp32 ones, and what a weight of less than 2^-30 of its row's largest loses is below 2^-30 of the value that it
+ * keep 22 bits or more: relative to each factor over 16-bit caches (over fp16 ones a query value below 2^-17 of its row's
+ * largest loses up to 2^-39 of that largest), to the largest value of its row of the cache over fp32 ones (if that is at
+ * least 2^-122), and what a weight of less than 2^-30 of its row's largest loses is below 2^-30 of the value that it
  * weighs.  With bf16 activations the softmax weights are rounded to 16 bits (the cache's type; fp16 for fp32 caches)
  * for the second product.
  * chunks->rows * heads / 16 + chunks->n * kv_heads must be below 2^23. */
