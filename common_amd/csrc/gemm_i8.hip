@@ -46,16 +46,26 @@ __device__ inline float gated(float g, float u) {
     }
 }
 
-// One output from the sums over W (and W2).  Every kernel ends in these operations and no others, so that a row's bits do
-// not depend on the batch.
-template <int EPI, class CT>
-__device__ inline float finished(float sa, float sw, float sw2, float more, int g, int u) {
+// sa * sw * sum (+ more).  sa * sum may be past fp32 where the product is not, from token scales of kFarScale on (sums are below
+// 2^31 in magnitude): FAR takes it 2^64 times smaller then, which is the same to the last bit but for what fp32 cannot hold.
+constexpr float kFarScale = 0x1p96f;
+template <bool FAR, bool ADD>
+__device__ inline float scaled(int sum, float sa, float sw, float more) {
 #pragma clang fp contract(off)
-    const float v = (float)g * sa;
+    const float v = (float)sum * sa, near = ADD ? fmaf(v, sw, more) : v * sw;
+    if constexpr (!FAR) return near;
+    const float less = (float)sum * (sa * 0x1p-64f) * sw;
+    return fabsf(v) < INFINITY ? near : ADD ? fmaf(less, 0x1p64f, more) : less * 0x1p64f;
+}
+
+// One output from the sums over W (and W2).  Every kernel ends in these operations and no others, so that a row's bits do
+// not depend on the batch.  FAR: token scales may be above kFarScale.
+template <int EPI, class CT, bool FAR>
+__device__ inline float finished(float sa, float sw, float sw2, float more, int g, int u) {
     if constexpr (EPI == GEMV_EPI_SWIGLU) {
-        return gated<sizeof(CT) == 4>(v * sw, (float)u * sa * sw2);
+        return gated<sizeof(CT) == 4>(scaled<FAR, false>(g, sa, sw, 0.f), scaled<FAR, false>(u, sa, sw2, 0.f));
     } else {
-        return fmaf(v, sw, more);  // more: the bias, the residual or nothing
+        return scaled<FAR, true>(g, sa, sw, more);  // more: the bias, the residual or nothing
     }
 }
 
@@ -118,7 +128,7 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(I8Params p) {
         float more = 0.f;
         if constexpr (EPI == GEMV_EPI_STORE) more = p.bias ? p.bias[n + i] : 0.f;
         if constexpr (EPI == GEMV_EPI_RESIDUAL) more = to_float<CT>(c[i]);
-        out[q] = finished<EPI, CT>(p.sa[r], p.sw[n + i], NW == 2 ? p.sw2[n + i] : 0.f, more, acc[0][q], acc[NW - 1][q]);
+        out[q] = finished<EPI, CT, true>(p.sa[r], p.sw[n + i], NW == 2 ? p.sw2[n + i] : 0.f, more, acc[0][q], acc[NW - 1][q]);
     }
 #pragma unroll
     for (int q = 0; q < 4; q++)
@@ -193,26 +203,37 @@ __device__ constexpr int token_of(int r) { return (r >> 2) * 8 + (r & 3); }
 // outputs that do not exist get an offset past the buffer's end, where loads give zero and stores do nothing.  Without
 // branches: a load that some path does not use makes the compiler wait for all loads, the copies among them, wherever its
 // register is used next, which was in the loop over k (1,024 x 2,560 over 4,096 25 us instead of 19).
-// pair: all outputs exist and two bf16 ones fit a 4-byte store.
+// pair: all outputs exist and two bf16 ones fit a 4-byte store.  far: one of the tokens' scales is above kFarScale.
 template <int EPI, class CT, class Sums>
-__device__ inline void store_32x32(const I8Params& p, int m0, int n0, bool pair, const float (&sa)[16], float sw, float sw2,
-                                   float bias, const Sums& g, const Sums& u) {
+__device__ inline void store_32x32(const I8Params& p, int m0, int n0, bool pair, bool far, const float (&sa)[16], float sw,
+                                   float sw2, float bias, const Sums& g, const Sums& u) {
     const __amdgpu_buffer_rsrc_t c = buffer_of((CT*)p.c + (size_t)m0 * p.ldc + n0);
     const int lane = threadIdx.x & 63, first = (lane >> 5) * 4, bytes = (int)p.ldc * (int)sizeof(CT);
     const int at = first * bytes + (lane & 31) * (int)sizeof(CT);
     const int tokens = n0 + (lane & 31) < p.N ? p.M - m0 - first : 0;  // that the lane's output has
-    auto place = [&](int r) { return token_of(r) < tokens ? at : kNoOffset; };
+    auto place = [&](int r, int tokens, int at) { return token_of(r) < tokens ? at : kNoOffset; };
+    auto more = [&](int r, int tokens, int at) {
+        if constexpr (EPI != GEMV_EPI_RESIDUAL) return bias;
+        else if constexpr (sizeof(CT) == 4)
+            return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(c, place(r, tokens, at), token_of(r) * bytes, 0));
+        else
+            return to_float<CT>(__builtin_amdgcn_raw_buffer_load_b16(c, place(r, tokens, at), token_of(r) * bytes, 0));
+    };
     float out[16];
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        if constexpr (EPI != GEMV_EPI_RESIDUAL) out[r] = bias;
-        else if constexpr (sizeof(CT) == 4)
-            out[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(c, place(r), token_of(r) * bytes, 0));
-        else
-            out[r] = to_float<CT>(__builtin_amdgcn_raw_buffer_load_b16(c, place(r), token_of(r) * bytes, 0));
-    }
+    for (int r = 0; r < 16; r++) out[r] = more(r, tokens, at);
 #pragma unroll
-    for (int r = 0; r < 16; r++) out[r] = finished<EPI, CT>(sa[r], sw, sw2, out[r], g[r], u[r]);
+    for (int r = 0; r < 16; r++) out[r] = finished<EPI, CT, false>(sa[r], sw, sw2, out[r], g[r], u[r]);
+    if (far) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            // (hidden, or what both have in common would be computed, and held, ahead of the branch)
+            int sum = g[r], sum2 = u[r], left = tokens, first_at = at;
+            asm volatile("" : "+v"(sum), "+v"(sum2), "+v"(left), "+v"(first_at)::"memory");
+            __builtin_amdgcn_sched_barrier(0);
+            out[r] = finished<EPI, CT, true>(sa[r], sw, sw2, more(r, left, first_at), sum, sum2);
+        }
+    }
     if constexpr (sizeof(CT) == 2) {
         if (pair) {  // neighbouring lanes swap one of two tokens' values: each stores two outputs of one token
             typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -230,21 +251,25 @@ __device__ inline void store_32x32(const I8Params& p, int m0, int n0, bool pair,
             return;
         }
     }
+    int from = at;
+    if constexpr (sizeof(CT) == 2) asm volatile("" : "+v"(from));  // (places anew, instead of 16 registers for the loads' ones)
 #pragma unroll
     for (int r = 0; r < 16; r++) {
         if constexpr (sizeof(CT) == 4)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out[r]), c, place(r), token_of(r) * bytes, 0);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out[r]), c, place(r, tokens, from), token_of(r) * bytes, 0);
         else
-            __builtin_amdgcn_raw_buffer_store_b16(from_float<CT>(out[r]), c, place(r), token_of(r) * bytes, 0);
+            __builtin_amdgcn_raw_buffer_store_b16(from_float<CT>(out[r]), c, place(r, tokens, from), token_of(r) * bytes, 0);
     }
 }
 template <class CT>
 __device__ inline bool pairs_fit(const I8Params& p) {
     return (reinterpret_cast<uintptr_t>(p.c) & 3) == 0 && p.ldc % 2 == 0;
 }
-__device__ inline void token_scales(const I8Params& p, int m0, float (&sa)[16]) {
+// The scales of a lane's 16 tokens from m0 on; true where one of the wavefront's 32 is above kFarScale.
+__device__ inline bool token_scales(const I8Params& p, int m0, float (&sa)[16]) {
     typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-    const int first = (threadIdx.x & 63) >> 5 << 2;
+    const int lane = threadIdx.x & 63, first = lane >> 5 << 2;
+    const float one = p.sa[min(m0 + (lane & 31), p.M - 1)];  // (a token a lane: one comparison looks at all of them)
     if (m0 + 32 <= p.M) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -256,6 +281,7 @@ __device__ inline void token_scales(const I8Params& p, int m0, float (&sa)[16]) 
 #pragma unroll
         for (int r = 0; r < 16; r++) sa[r] = p.sa[min(m0 + first + token_of(r), p.M - 1)];
     }
+    return __builtin_amdgcn_ballot_w64(fabsf(one) > kFarScale) != 0;
 }
 #endif
 
@@ -450,11 +476,11 @@ __global__ __launch_bounds__(T::WAVES * 64, T::PER_CU * T::WAVES / 4) void gemm_
 #pragma unroll
             for (int i = 0; i < T::FM; i++) {
                 float sa[16];
-                token_scales(p, mw + i * 32, sa);
+                const bool far = token_scales(p, mw + i * 32, sa);
 #pragma unroll
                 for (int j = 0; j < T::FN; j++) {
-                    store_32x32<T::EPI, CT>(p, mw + i * 32, nw + j * 32, pair, sa, sw[j], sw2[j], bias[j], acc[0][i][j],
-                                            acc[T::NW - 1][i][j]);
+                    store_32x32<T::EPI, CT>(p, mw + i * 32, nw + j * 32, pair, far, sa, sw[j], sw2[j], bias[j],
+                                            acc[0][i][j], acc[T::NW - 1][i][j]);
                     __builtin_amdgcn_sched_barrier(0);  // (what all 32 x 32 read would not fit the registers at once)
                 }
             }
@@ -495,8 +521,8 @@ __global__ __launch_bounds__(256) void gemm_i8_sum_kernel(I8Params p, Cut cut) {
     }
     const int n = min(n0 + (lane & 31), p.N - 1);
     float sa[16];
-    token_scales(p, m0, sa);
-    store_32x32<T::EPI, CT>(p, m0, n0, m0 + 32 <= p.M && n0 + 32 <= p.N && pairs_fit<CT>(p), sa, p.sw[n],
+    const bool far = token_scales(p, m0, sa);
+    store_32x32<T::EPI, CT>(p, m0, n0, m0 + 32 <= p.M && n0 + 32 <= p.N && pairs_fit<CT>(p), far, sa, p.sw[n],
                             T::NW == 2 ? p.sw2[n] : 0.f, T::EPI == GEMV_EPI_STORE && p.bias ? p.bias[n] : 0.f, sum[0],
                             sum[T::NW - 1]);
 #endif

@@ -1,0 +1,89 @@
+"""GPU checks of the 8-bit path at the ends of fp32's range, against numpy in 64 bits.
+
+Tolerances, u = 2^-24, r the half step of the result's type (bf16 2^-8, fp32 u), relative, for results that are normal numbers:
+  product: the sum's conversion and the two products by scales u each, bias and residual u of the result, then r; gated
+      (6 |gate| + 32) u of the result in all, then r (test_gpu_int8.py derives both).
+"""
+import numpy as np
+import pytest
+
+import int8_reference as ref
+from int8_reference import HALF, U
+from test_gpu_int8 import Floats, Eights, Product, CODE, EPILOGUE, ops  # noqa: F401 (ops: the fixture)
+
+pytestmark = pytest.mark.gpu
+NORMAL = 2.0 ** -126  # the smallest normal number of fp32 and bf16
+
+
+def _scales(e, values):
+    e.sbuf.upload(np.ascontiguousarray(values, np.float32))
+
+
+def _far_scales(p, r):
+    """Scales of tokens from 2^97 on, of outputs so small that the products are ordinary numbers: scaleA * sum is past fp32 for
+    many of them, scaleA * scaleW * sum for none.  Every third token stays ordinary.  Gated: gates of up to some tens."""
+    gated = p.epilogue == "gated"
+    sa = np.ldexp(r.uniform(1, 1.99, p.m), r.integers(97, 112 if gated else 128, p.m))
+    sa[1::3] = r.uniform(0.5, 2, len(sa[1::3]))
+    if p.m > 4:
+        sa[3] = -sa[3]
+    _scales(p.a, sa)
+    _scales(p.w, np.ldexp(r.uniform(1, 2, p.n), r.integers(-126, -124 if gated else -100, p.n)))
+    if gated:
+        _scales(p.w2, np.ldexp(r.uniform(1, 2, p.n), r.integers(-126, -100, p.n)))
+
+
+FAR = [(1, 2560, 4096), (3, 40, 64), (16, 100, 300), (20, 5000, 200), (64, 512, 1024), (100, 260, 500), (300, 700, 640),
+       (700, 5000, 300), (64, 2560, 9728)]
+
+
+@pytest.mark.parametrize("m,n,k", FAR)
+@pytest.mark.parametrize("epilogue,out", [("store", "f32"), ("residual", "bf16"), ("gated", "f32"), ("gated", "bf16")])
+def test_token_scales_near_fp32s_largest(ctx, ops, m, n, k, epilogue, out):  # noqa: F811
+    """scaleA * sum may be past fp32 where scaleA * scaleW * sum is not."""
+    r = np.random.default_rng([m, n, k])
+    p = Product(ctx, m, n, k, epilogue, out, bias=epilogue == "store")
+    _far_scales(p, r)
+    p.run(ops)
+    ctx.synchronize()
+    sa = p.scales(p.a)[:, None]
+    g = ref.sums(p.aq, p.wq) * sa * p.scales(p.w)
+    near = np.abs(g) <= 80  # (of the gated ones)
+    if epilogue == "gated":
+        want = np.where(near, ref.sums(p.aq, p.w2q) * sa * p.scales(p.w2) * ref.silu(np.where(near, g, 0)), 0)
+        off = (6 * np.abs(g) + 32) * U * np.abs(want)
+    else:
+        more = p.c.values.astype(np.float64) if epilogue == "residual" else p.bias.values.astype(np.float64)
+        want = g + more
+        off = 3 * U * np.abs(g) + U * np.abs(want)
+    off = off + (HALF[out] if out != "f32" else 0) * (np.abs(want) + off) + NORMAL
+    got = p.c.get().astype(np.float64)
+    look = near if epilogue == "gated" else np.ones_like(near)
+    assert look.mean() > 0.5 and np.abs(want).max() < 2.0 ** 100
+    assert (np.abs(got - want) <= off * (1 + 8 * U))[look].all()
+
+
+@pytest.mark.parametrize("epilogue,out", [("store", "f32"), ("residual", "bf16"), ("gated", "f32"), ("gated", "bf16")])
+def test_rows_beside_such_tokens_have_the_same_bits(ctx, ops, epilogue, out):  # noqa: F811
+    p = Product(ctx, 150, 300, 700, epilogue, out, bias=epilogue == "store", seed=3)
+    plain = p.scales(p.a)
+    sa = plain.copy()
+    sa[::5] = 2.0 ** 127
+    _scales(p.a, np.concatenate([sa, [5.0]]))
+    p.run(ops)
+    ctx.synchronize()
+    got = p.c.get()
+    keep = np.arange(150) % 5 != 0
+    for rows in (np.nonzero(keep)[0][:7], np.nonzero(keep)[0][:60], np.nonzero(keep)[0]):
+        c = Floats(ctx, p.c.values[rows], out)
+        a = Eights(ctx, len(rows), 700, 0, p.aq[rows], plain[rows])
+        ops.gemm(a.raw, p.w.raw, c, epilogue=EPILOGUE[epilogue], W2=p.w2.raw if p.w2 else None, bias=p.bias,
+                 c_dtype=CODE[out])
+        ctx.synchronize()
+        assert (c.get() == got[rows]).all()
+    far = got[~keep]
+    alone = Floats(ctx, p.c.values[~keep], out)
+    a = Eights(ctx, 30, 700, 0, p.aq[~keep], sa[~keep])
+    ops.gemm(a.raw, p.w.raw, alone, epilogue=EPILOGUE[epilogue], W2=p.w2.raw if p.w2 else None, bias=p.bias, c_dtype=CODE[out])
+    ctx.synchronize()
+    assert np.array_equal(alone.get(), far, equal_nan=True)
