@@ -23,16 +23,15 @@ struct I8Params {
     int64_t ldc;
 };
 
-// up * silu(gate).  EXACT (fp32 outputs): from e = exp(-|gate|), which does not overflow: silu = gate / (1 + e), times e for
-// gates below 0; e is the square of 2^(t/2), t = -|gate| log2(e), which reaches twice as far down as the hardware's 2^t,
-// corrected by the rounding error of t, and the quotient is corrected by one step: to about 2^-23.  bf16 outputs: the bare
-// reciprocal of 1 + 2^t, t = -gate log2(e), some |gate| 2^-23 off, far below half a step of bf16.  Gates further down than
-// -128 (bf16: -87, whose silu is below 2^-118) count as that, minus infinity among them; NaN stays.
+// up * silu(gate) for gates from kFarGate on, and NaN.  EXACT (fp32 outputs): from e = exp(-|gate|), which does not overflow:
+// silu = gate / (1 + e), times e for gates below 0; e is the square of 2^(t/2), t = -|gate| log2(e), which reaches twice as far
+// down as the hardware's 2^t, corrected by the rounding error of t, and the quotient is corrected by one step: to about 2^-23.
+// bf16 outputs: the bare reciprocal of 1 + 2^t, t = -gate log2(e), some |gate| 2^-23 off, far below half a step of bf16.
+constexpr float kFarGate = -87.f;
 template <bool EXACT>
 __device__ inline float gated(float g, float u) {
 #pragma clang fp contract(off)
     if constexpr (EXACT) {
-        g = __builtin_elementwise_maximum(g, -128.f);  // (v_maximum3_f32: NaN if one of them is)
         const float a = fminf(fabsf(g), 128.f), t = a * -1.44269502f;
         const float s = __builtin_amdgcn_exp2f(0.5f * t);
         const float d = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, -a));  // ln 2 = 0.693147182 - 1.904654e-9
@@ -41,9 +40,19 @@ __device__ inline float gated(float g, float u) {
         const float r = __builtin_amdgcn_rcpf(den), q = num * r;
         return u * (q < INFINITY ? fmaf(fmaf(-den, q, num), r, q) : q);
     } else {
-        g = __builtin_elementwise_maximum(g, -87.f);
         return u * (g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269502f)));
     }
+}
+
+// ... and for gates below kFarGate, whose silu = gate * e, e = exp(gate), need not be a normal number where its product with
+// `up` is one: e is the fourth power of 2^(t/4), two of which go to the gate and two to `up`, corrected as above.  Gates below
+// -300, minus infinity among them, count as that, where two are 0.
+__device__ inline float gated_far(float g, float u) {
+#pragma clang fp contract(off)
+    g = fmaxf(g, -300.f);
+    const float t = g * 1.44269502f, s = __builtin_amdgcn_exp2f(0.25f * t);
+    const float d = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, g)), v = u * s * s * (g * s * s);
+    return fmaf(v, d, v);
 }
 
 // sa * sw * sum (+ more).  sa * sum may be past fp32 where the product is not, from token scales of kFarScale on (sums are below
@@ -59,11 +68,14 @@ __device__ inline float scaled(int sum, float sa, float sw, float more) {
 }
 
 // One output from the sums over W (and W2).  Every kernel ends in these operations and no others, so that a row's bits do
-// not depend on the batch.  FAR: token scales may be above kFarScale.
+// not depend on the batch.  FAR: token scales may be above kFarScale, gates below kFarGate.
 template <int EPI, class CT, bool FAR>
 __device__ inline float finished(float sa, float sw, float sw2, float more, int g, int u) {
     if constexpr (EPI == GEMV_EPI_SWIGLU) {
-        return gated<sizeof(CT) == 4>(scaled<FAR, false>(g, sa, sw, 0.f), scaled<FAR, false>(u, sa, sw2, 0.f));
+        const float gate = scaled<FAR, false>(g, sa, sw, 0.f), up = scaled<FAR, false>(u, sa, sw2, 0.f);
+        const float near = gated<sizeof(CT) == 4>(gate, up);
+        if constexpr (!FAR) return near;
+        return gate < kFarGate ? gated_far(gate, up) : near;
     } else {
         return scaled<FAR, true>(g, sa, sw, more);  // more: the bias, the residual or nothing
     }
@@ -121,14 +133,26 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(I8Params p) {
     const int n = n0 + (lane >> 4) * 4, last = p.N - 1 - n;
     if (r >= p.M || last < 0) return;
     CT* const c = (CT*)p.c + (size_t)r * p.ldc + n;
-    float out[4];
+    const float sa = p.sa[r];
+    float out[4], sw[4], sw2[4], more[4], least = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         const int i = min(q, last);
-        float more = 0.f;
-        if constexpr (EPI == GEMV_EPI_STORE) more = p.bias ? p.bias[n + i] : 0.f;
-        if constexpr (EPI == GEMV_EPI_RESIDUAL) more = to_float<CT>(c[i]);
-        out[q] = finished<EPI, CT, true>(p.sa[r], p.sw[n + i], NW == 2 ? p.sw2[n + i] : 0.f, more, acc[0][q], acc[NW - 1][q]);
+        sw[q] = p.sw[n + i];
+        sw2[q] = NW == 2 ? p.sw2[n + i] : 0.f;
+        more[q] = 0.f;
+        if constexpr (EPI == GEMV_EPI_STORE) more[q] = p.bias ? p.bias[n + i] : 0.f;
+        if constexpr (EPI == GEMV_EPI_RESIDUAL) more[q] = to_float<CT>(c[i]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        out[q] = finished<EPI, CT, false>(sa, sw[q], sw2[q], more[q], acc[0][q], acc[NW - 1][q]);
+        if constexpr (NW == 2) least = fminf(least, scaled<false, false>(acc[0][q], sa, sw[q], 0.f));
+    }
+    if (fabsf(sa) > kFarScale || least < kFarGate) {
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            out[q] = finished<EPI, CT, true>(sa, sw[q], sw2[q], more[q], acc[0][q], acc[NW - 1][q]);
     }
 #pragma unroll
     for (int q = 0; q < 4; q++)
@@ -224,6 +248,12 @@ __device__ inline void store_32x32(const I8Params& p, int m0, int n0, bool pair,
     for (int r = 0; r < 16; r++) out[r] = more(r, tokens, at);
 #pragma unroll
     for (int r = 0; r < 16; r++) out[r] = finished<EPI, CT, false>(sa[r], sw, sw2, out[r], g[r], u[r]);
+    if constexpr (EPI == GEMV_EPI_SWIGLU) {
+        float least = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) least = fminf(least, scaled<false, false>(g[r], sa[r], sw, 0.f));
+        far = far || __builtin_amdgcn_ballot_w64(least < kFarGate) != 0;
+    }
     if (far) {
 #pragma unroll
         for (int r = 0; r < 16; r++) {

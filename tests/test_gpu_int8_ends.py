@@ -87,3 +87,45 @@ def test_rows_beside_such_tokens_have_the_same_bits(ctx, ops, epilogue, out):  #
     ops.gemm(a.raw, p.w.raw, alone, epilogue=EPILOGUE[epilogue], W2=p.w2.raw if p.w2 else None, bias=p.bias, c_dtype=CODE[out])
     ctx.synchronize()
     assert np.array_equal(alone.get(), far, equal_nan=True)
+
+
+@pytest.mark.parametrize("m", [1, 12, 40, 130, 300])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_gates_far_below_zero_before_large_up_projections(ctx, ops, m, out):  # noqa: F811
+    """silu(-100) is 100 * 2^-144: no normal number of fp32, but the product with an up projection of 1e30 is."""
+    r = np.random.default_rng(m)
+    n, k = 200, 128
+    p = Product(ctx, m, n, k, "gated", out)
+    sa = np.exp(r.uniform(-1, 1, m))
+    _scales(p.a, sa)
+    sums, sums2 = ref.sums(p.aq, p.wq), ref.sums(p.aq, p.w2q)
+    _scales(p.w, np.exp(r.uniform(np.log(20), np.log(400), n)) / np.abs(sums).mean())  # gates to some -1,000
+    _scales(p.w2, np.ldexp(r.uniform(1, 2, n), r.integers(0, 100, n)))
+    p.run(ops)
+    ctx.synchronize()
+    g = sums * p.scales(p.a)[:, None] * p.scales(p.w)
+    up = sums2 * p.scales(p.a)[:, None] * p.scales(p.w2)
+    want = up * ref.silu(g)
+    off = (6 * np.abs(g) + 32) * U * np.abs(want)
+    off = off + (HALF[out] if out != "f32" else 0) * (np.abs(want) + off) + NORMAL
+    far = (g < -87) & (np.abs(want) > 2.0 ** -100)
+    assert far.sum() > 5
+    got = p.c.get().astype(np.float64)
+    past = np.abs(want) > 2.0 ** 128  # (what is past both types' largest is infinite)
+    assert (got[past] == np.sign(want[past]) * np.inf).all()
+    bad = ~past & ~(np.abs(got - want) <= off * (1 + 8 * U))
+    assert not bad.any(), (int(bad.sum()), g[bad][:5], up[bad][:5], got[bad][:5], want[bad][:5])
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_gates_of_minus_infinity_shut_the_up_projection_off(ctx, ops, m, out):  # noqa: F811
+    n, k = 96, 256
+    one = np.ones((m, k), np.int8)
+    a = Eights(ctx, m, k, 0, one, np.ones(m, np.float32))
+    w = Eights(ctx, n, k, 0, -np.ones((n, k), np.int8), np.full(n, 3e38, np.float32))
+    w2 = Eights(ctx, n, k, 0, np.ones((n, k), np.int8), np.full(n, 1e35, np.float32))
+    c = Floats(ctx, np.ones((m, n)), out)
+    ops.gemm(a.raw, w.raw, c, epilogue=EPILOGUE["gated"], W2=w2.raw, c_dtype=CODE[out])
+    ctx.synchronize()
+    assert (c.get() == 0).all()
