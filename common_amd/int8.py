@@ -18,6 +18,7 @@ that needs more work space than any before it allocates it; the space that queue
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 from .hardware import DTYPE_F32, GEMM_STORE, HipContext, check, lib
 
@@ -40,7 +41,7 @@ class Int8Rows:
     def __init__(self, ctx: HipContext, rows: int, n: int, q=None, scale=None, stride: int = 0):
         self.ctx, self.rows, self.n = ctx, rows, n
         self.stride = stride or -(-n // 16) * 16
-        self._own = []
+        self._own, self._parts = [], weakref.WeakSet()
         try:
             self.q = q if q is not None else self._take(rows * self.stride)
             self.scale = scale if scale is not None else self._take(rows * 4)
@@ -59,13 +60,17 @@ class Int8Rows:
         self.ref = ctypes.byref(self.raw)
 
     def first(self, rows: int) -> "Int8Rows":
-        """The first `rows` rows, on the same buffers."""
+        """The first `rows` rows, on the same buffers; they end with these."""
         if not 0 <= rows <= self.rows:
             raise ValueError(f"{rows} of {self.rows} rows")
-        return Int8Rows(self.ctx, rows, self.n, self.q, self.scale, self.stride)
+        part = Int8Rows(self.ctx, rows, self.n, self.q, self.scale, self.stride)
+        self._parts.add(part)
+        return part
 
     def close(self):
-        """Frees the buffers these rows allocated."""
+        """Frees the buffers these rows allocated; calls with them, or with rows taken from them, are refused after it."""
+        for part in list(self._parts):
+            part.close()
         for buf in self._own:
             buf.free()
         self._own = []

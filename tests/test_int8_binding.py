@@ -1,0 +1,50 @@
+"""CPU checks of what common_amd.int8 does before and after the C calls."""
+import pytest
+
+from common_amd import hardware as hw
+from common_amd import int8
+
+
+class _Buf:
+    def __init__(self, ptr):
+        self.ptr, self.freed = ptr, False
+
+    def free(self):
+        self.freed, self.ptr = True, None
+
+
+class _Context:
+    """A context of device `index` that never reaches one: calls that get past the binding are refused by the library."""
+
+    handle = None
+
+    def __init__(self, index=0):
+        self.index, self.bufs = index, []
+
+    def allocate(self, nbytes):
+        self.bufs.append(_Buf(4096 * (len(self.bufs) + 1)))
+        return self.bufs[-1]
+
+
+def test_rows_taken_from_others_end_with_them():
+    """After `close` the memory is gone: rows that share it must not keep its address."""
+    ctx = _Context()
+    whole = int8.Int8Rows(ctx, 8, 40)
+    part = whole.first(5)
+    less = part.first(2)
+    assert part.raw.q == less.raw.q == whole.raw.q and (part.raw.rows, less.raw.rows) == (5, 2)
+    part.close()  # (its own are none: the others stay)
+    assert part.raw.q is None and less.raw.q is None and whole.raw.q == 4096 and not any(b.freed for b in ctx.bufs)
+    again, kept = whole.first(8), whole.first(3)
+    whole.close()
+    assert all(b.freed for b in ctx.bufs)
+    for rows in (whole, again, kept):
+        assert rows.raw.q is None and rows.raw.scale is None
+        with int8.Int8Ops(ctx) as ops, pytest.raises(hw.HardwareException, match="null pointer"):
+            ops.quantize(_Buf(4096), rows)
+
+
+def test_rows_outlive_the_ones_they_were_taken_from():
+    ctx = _Context()
+    part = int8.Int8Rows(ctx, 8, 40).first(5)
+    assert part.raw.q == 4096 and not any(b.freed for b in ctx.bufs)
