@@ -63,6 +63,8 @@ class Int8Rows:
         """The first `rows` rows, on the same buffers; they end with these."""
         if not 0 <= rows <= self.rows:
             raise ValueError(f"{rows} of {self.rows} rows")
+        if self.q is None:
+            raise ValueError("the rows are closed")
         part = Int8Rows(self.ctx, rows, self.n, self.q, self.scale, self.stride)
         self._parts.add(part)
         return part

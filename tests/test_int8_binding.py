@@ -48,3 +48,13 @@ def test_rows_outlive_the_ones_they_were_taken_from():
     ctx = _Context()
     part = int8.Int8Rows(ctx, 8, 40).first(5)
     assert part.raw.q == 4096 and not any(b.freed for b in ctx.bufs)
+
+
+def test_no_rows_are_taken_from_closed_ones():
+    """`first` of closed rows allocated new, unset memory for what it took."""
+    ctx = _Context()
+    whole = int8.Int8Rows(ctx, 8, 40)
+    whole.close()
+    with pytest.raises(ValueError, match="closed"):
+        whole.first(3)
+    assert len(ctx.bufs) == 2
