@@ -12,7 +12,8 @@ No counterpart in the reference (its contexts compute in FP32 or FP64).  A feed-
     ops.quantize(act, act8)
     ops.gemm(act8, down, h, epilogue=GEMM_RESIDUAL)                          # h += down
 
-Buffers are anything with a ``ptr`` (``hardware.DeviceBuffer``).  Everything runs on the context's stream.  A product
+Buffers are anything with a ``ptr`` (``hardware.DeviceBuffer``).  Everything runs on the context's stream.  Rows of another
+context on the same device may be used (the order between the two streams is the caller's), of another device not.  A product
 that needs more work space than any before it allocates it; the space that queued calls still use stays until ``close``.
 """
 from __future__ import annotations
@@ -102,12 +103,17 @@ class Int8Ops:
     def __exit__(self, *exc):
         self.close()
 
+    def _check_device(self, rows: Int8Rows):
+        if rows.ctx is not self.ctx and rows.ctx.index != self.ctx.index:
+            raise ValueError(f"rows of device {rows.ctx.index} cannot be used on device {self.ctx.index}")
+
     def rows(self, rows: int, n: int) -> Int8Rows:
         """New rows in 8 bits."""
         return Int8Rows(self.ctx, rows, n)
 
     def quantize(self, x, out: Int8Rows, x_dtype: int = DTYPE_F32, x_stride: int = 0):
         """Rows of floats to 8 bits (ar_hip_quantize_i8).  A stride of 0, here and below: rows one after another."""
+        self._check_device(out)
         rc = self._quantize(self.ctx.handle, _ptr(x), x_dtype, x_stride or out.n, out.ref)
         if rc:
             check(rc)
@@ -124,6 +130,7 @@ class Int8Ops:
     def add_rmsnorm_i8(self, h, w, eps: float, out: Int8Rows, x=None, h_dtype: int = DTYPE_F32,
                        x_dtype: int = DTYPE_F32, h_stride: int = 0, x_stride: int = 0):
         """h += x, out = rmsnorm(h) * w in 8 bits (ar_hip_add_rmsnorm_i8)."""
+        self._check_device(out)
         rc = self._norm_i8(self.ctx.handle, _ptr(h), h_dtype, h_stride or out.n, _ptr(x), x_dtype, x_stride or out.n, _ptr(w),
                            eps, out.ref)
         if rc:
@@ -131,6 +138,7 @@ class Int8Ops:
 
     def embed(self, table: Int8Rows, tokens, count: int, y, y_dtype: int = DTYPE_F32, y_stride: int = 0):
         """Rows of the table by token (None: the first `count`) as floats (ar_hip_embed_i8)."""
+        self._check_device(table)
         rc = self._embed(self.ctx.handle, table.ref, _ptr(tokens), count, _ptr(y), y_dtype, y_stride or table.n)
         if rc:
             check(rc)
@@ -155,6 +163,10 @@ class Int8Ops:
     def gemm(self, A: Int8Rows, W: Int8Rows, C, epilogue: int = GEMM_STORE, W2: Int8Rows | None = None, bias=None,
              c_dtype: int = DTYPE_F32, ldc: int = 0):
         """C = A W^T, C += A W^T or C = (A W2^T) * silu(A W^T) of rows in 8 bits (ar_hip_gemm_i8)."""
+        self._check_device(A)
+        self._check_device(W)
+        if W2 is not None:
+            self._check_device(W2)
         w = self._scratch(A.rows, W.rows, A.n, epilogue)
         rc = self._gemm(self.ctx.handle, A.ref, W.ref, W2.ref if W2 is not None else None, _ptr(bias), _ptr(C), c_dtype,
                         ldc or W.rows, epilogue, _ptr(w), w.nbytes if w else 0)

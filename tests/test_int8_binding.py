@@ -58,3 +58,25 @@ def test_no_rows_are_taken_from_closed_ones():
     with pytest.raises(ValueError, match="closed"):
         whole.first(3)
     assert len(ctx.bufs) == 2
+
+
+CALLS = {
+    "quantize": lambda ops, rows, other: ops.quantize(_Buf(4096), other),
+    "add_rmsnorm_i8": lambda ops, rows, other: ops.add_rmsnorm_i8(_Buf(4096), _Buf(4096), 1e-6, other),
+    "embed": lambda ops, rows, other: ops.embed(other, None, 2, _Buf(4096)),
+    "gemm A": lambda ops, rows, other: ops.gemm(other, rows, _Buf(4096)),
+    "gemm W": lambda ops, rows, other: ops.gemm(rows, other, _Buf(4096)),
+    "gemm W2": lambda ops, rows, other: ops.gemm(rows, rows, _Buf(4096), epilogue=hw.GEMM_SWIGLU, W2=other),
+}
+
+
+@pytest.mark.parametrize("call", sorted(CALLS))
+def test_rows_of_another_device_are_refused(call):
+    """Their memory is another GPU's; rows of another context on the same device are the caller's to order."""
+    ops = int8.Int8Ops(_Context(0))
+    rows = int8.Int8Rows(ops.ctx, 8, 40)
+    with pytest.raises(ValueError, match="rows of device 1 .* device 0"):
+        CALLS[call](ops, rows, int8.Int8Rows(_Context(1), 8, 40))
+    assert len(ops.ctx.bufs) == 2  # (no work space was taken for it)
+    with pytest.raises(hw.HardwareException, match="ctx is null"):
+        CALLS[call](ops, rows, int8.Int8Rows(_Context(0), 8, 40))
