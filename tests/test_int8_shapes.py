@@ -1,0 +1,62 @@
+"""CPU check that the products of int8_shapes.py, which the GPU tests run, go to every kernel that the rule for tiles comes to: a
+rule that is changed without them fails here."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from int8_shapes import GATED, STORED
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ROWS = 7  # the kind of the kernel that takes its operands straight from memory
+
+
+@pytest.fixture(scope="module")
+def launches(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    exe = str(tmp_path_factory.mktemp("reach") / "i8_reach")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-o", exe,
+                    os.path.join(ROOT, "tests", "sanitize", "i8_reach_main.cpp")], check=True)
+
+    def run(*args):
+        r = subprocess.run([exe, *args], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+        return [tuple(int(v) for v in line.split()) for line in r.stdout.splitlines()]
+
+    return run
+
+
+def _shapes(gated):
+    return GATED if gated else STORED
+
+
+def test_every_launch_that_the_rule_comes_to_is_among_the_tested_ones(launches):
+    reached = {(g, kind, parts > 1, rounds if parts == 1 else 0) for g, kind, parts, rounds in launches()}
+    tested = set()
+    for gated in (0, 1):
+        for (m, n, k), (g, kind, parts, rounds) in zip(_shapes(gated), launches(*[f"{m},{n},{k},{gated}" for m, n, k in _shapes(gated)])):
+            assert g == gated
+            tested.add((g, kind, parts > 1, rounds if parts == 1 else 0))
+    assert {x[:3] for x in reached} >= {(g, kind, False) for g in (0, 1) for kind in (0, 1, 3, 4, 6, ROWS)}
+    assert not reached - tested, sorted(reached - tested)
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+def test_parts_few_and_many(launches, gated):
+    """Of the kinds that take k in parts: few and many of them, in one round and in more."""
+    found = launches(*[f"{m},{n},{k},{gated}" for m, n, k in _shapes(gated)])
+    kinds = {kind for g, kind, parts, rounds in launches() if g == gated and parts > 1}
+    for kind in kinds:
+        parts = {x[2] for x in found if x[1] == kind and x[2] > 1}
+        assert min(parts) <= 4 and max(parts) >= 6, (kind, parts)
+    assert any(x[2] > 1 and x[3] > 1 for x in found)
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+def test_shapes_are_cut_by_every_edge(launches, gated):
+    for m, n, k in _shapes(gated):
+        k16 = -(-k // 16) * 16
+        assert k16 // 128 >= 8 and k16 % 128 and k % 16 and n % 32, (m, n, k)
+        assert m <= 32 or m % 32, (m, n, k)
