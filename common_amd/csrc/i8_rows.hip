@@ -41,6 +41,14 @@ __device__ inline unsigned row_max(unsigned v, unsigned* red, int waves) {
     return t;
 }
 
+// 1 / sqrt(mean of squares + eps) of a row whose squares' sum is ss.  Past 2^126 that is no normal number and short of bits:
+// `pre` (else 1) takes the values 2^64 times smaller first, which costs none that its product does not lose.
+__device__ inline float reciprocal_root(double ss, int n, float eps, float* pre) {
+    const double root = sqrt(ss / (double)n + (double)eps);
+    *pre = root > 0x1p126 ? 0x1p-64f : 1.f;
+    return (float)((root > 0x1p126 ? 0x1p64 : 1.0) / root);
+}
+
 // The magnitude's bits: ordered as the magnitudes are, infinities and NaN above every number.
 __device__ inline unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
@@ -150,7 +158,14 @@ __global__ __launch_bounds__(1024) void held_rows_kernel(RowParams p, int row0, 
         for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
             for (int j = 0; j < 8; j++) ss = fma((double)v[c][j], (double)v[c][j], ss);
-        const float rs = (float)(1.0 / sqrt(row_sum(ss, red_sum, waves) / (double)p.n + (double)p.eps));
+        float pre;
+        const float rs = reciprocal_root(row_sum(ss, red_sum, waves), p.n, p.eps, &pre);
+        if (pre != 1.f) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[c][j] *= pre;
+        }
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++) {
             const int i = (c * blockDim.x + threadIdx.x) * 8, left = p.n - i;
@@ -200,18 +215,18 @@ __global__ __launch_bounds__(256) void rows_kernel(RowParams p, int row0) {
         const float a = to_float<HT>(h[i]);
         return x ? a + to_float<XT>(x[i]) : a;
     };
-    float rs = 1.f;
+    float rs = 1.f, pre = 1.f;
     if constexpr (NORM) {
         double ss = 0.0;
         for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
             const float v = value(i);
             ss += (double)v * (double)v;
         }
-        rs = (float)(1.0 / sqrt(row_sum(ss, red_sum, blockDim.x >> 6) / (double)p.n + (double)p.eps));
+        rs = reciprocal_root(row_sum(ss, red_sum, blockDim.x >> 6), p.n, p.eps, &pre);
     }
     auto normed = [&](int i) {
         const float v = value(i);
-        return NORM ? v * rs * p.w[i] : v;
+        return NORM ? v * pre * rs * p.w[i] : v;
     };
     if constexpr (I8) {
         unsigned m = 0u;
@@ -230,7 +245,7 @@ __global__ __launch_bounds__(256) void rows_kernel(RowParams p, int row0) {
         // (y may be x: each thread reads an element of x and h before it writes there)
         YT* const y = (YT*)p.y + r * p.y_stride;
         for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
-            const float v = value(i), o = v * rs * p.w[i];
+            const float v = value(i), o = v * pre * rs * p.w[i];
             if (x) h[i] = from_float<HT>(v);
             y[i] = from_float<YT>(o);
         }

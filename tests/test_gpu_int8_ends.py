@@ -9,7 +9,7 @@ import pytest
 
 import int8_reference as ref
 from int8_reference import HALF, U
-from test_gpu_int8 import Floats, Eights, Product, CODE, EPILOGUE, ops  # noqa: F401 (ops: the fixture)
+from test_gpu_int8 import CODE, EPILOGUE, Eights, Floats, Product, _eights_agree, ops  # noqa: F401 (ops: the fixture)
 
 pytestmark = pytest.mark.gpu
 NORMAL = 2.0 ** -126  # the smallest normal number of fp32 and bf16
@@ -129,3 +129,27 @@ def test_gates_of_minus_infinity_shut_the_up_projection_off(ctx, ops, m, out):  
     ops.gemm(a.raw, w.raw, c, epilogue=EPILOGUE["gated"], W2=w2.raw, c_dtype=CODE[out])
     ctx.synchronize()
     assert (c.get() == 0).all()
+
+
+@pytest.mark.parametrize("n", [40, 2560, 40000])
+@pytest.mark.parametrize("yd", ["f32", "bf16", "i8"])
+def test_norms_of_rows_near_fp32s_largest(ctx, ops, n, yd):  # noqa: F811
+    """Root mean squares past 2^126, whose reciprocals are no normal numbers; within 5 u as all others (test_gpu_int8.py)."""
+    r = np.random.default_rng(n)
+    a = (r.uniform(2.6e38, 3.4e38, (33, n)) * r.choice([-1, 1], (33, n))).astype(np.float32)
+    a[::4, : n // 2] = 0
+    a[5] *= np.float32(2.0 ** -3)
+    a[6, 1:] = 1
+    h, w = Floats(ctx, a, "f32"), Floats(ctx, 1 + 0.3 * r.standard_normal((1, n)), "f32")
+    _, want = ref.norm(h.values, None, w.values[0], np.float32(1e-6))
+    if yd == "i8":
+        out = Eights(ctx, 33, n)
+        ops.add_rmsnorm_i8(h, w, 1e-6, out.raw)
+        ctx.synchronize()
+        _eights_agree(out, want, 5 * U)
+    else:
+        out = Floats(ctx, np.zeros((33, n)), yd)
+        ops.add_rmsnorm(h, w, 1e-6, 33, n, out, y_dtype=CODE[yd])
+        ctx.synchronize()
+        off = (5 * U + (HALF[yd] if yd != "f32" else 0)) * np.abs(want) * (1 + U) + NORMAL
+        assert (np.abs(out.get() - want) <= off).all()
