@@ -1,5 +1,5 @@
 // How products of rows in 8 bits are cut (common_amd/csrc/i8_plan.h), at every kind of size: a kernel that there is, parts of
-// at least four steps of k, work space for all of them, and no more rounds than the fewest tiles would take.
+// at least four steps of k, and work space for all of them.  (Which kernels sizes come to: i8_reach_main.cpp.)
 #include <cstdio>
 #include <cstdlib>
 #include <initializer_list>

@@ -308,7 +308,7 @@ def test_product(ctx, ops, m, n, k, epilogue, out, bias, strides):
     p.check()
 
 
-# tiles of every kind that the rule has, cut at the last token, output and step, in one round of the CUs and in several
+# larger tiles, cut at the last token, output and step, in one round of the CUs and in several (int8_shapes.py has every kind)
 LARGE = [(700, 5000, 300), (1025, 8200, 200), (2000, 6100, 150), (1500, 3000, 260), (515, 2600, 1100), (70, 1000, 9000),
          (140, 2500, 5000), (3000, 4100, 140), (4000, 4700, 160), (3900, 4500, 145), (900, 6000, 140), (2750, 9700, 200)]
 
