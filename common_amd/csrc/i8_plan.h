@@ -21,15 +21,18 @@ struct I8Plan {
 // What a product takes by each kind of tile, in us, up to what they have in common: tiles go in rounds of per_cu blocks a CU;
 // in a round a CU copies 70 KB a us, 128 bytes of k take 0.85 / (buffers - 1) us at least, the way from memory, and outputs
 // are finished one after the other.  Parts of k cost a launch and their sums' way through memory.  Fitted to 520 sizes by every
-// kind and number of parts (17 to 10,000 tokens, 768 to 20,000 outputs over 768 to 14,336, weights from memory), of which the
-// choice is 0.7% behind the fastest on average and more than 4.3% in one of 20 (MI355X).  Both sides of it, us: 509 x 2,560 over
-// 9,728 by 64 x 128 tiles 24.6, 128 x 128 32.2, 64 x 64 30.8; 448 x 2,048 over 6,144 by 64 x 64 17.2, 64 x 128 23.8; 1,024 x
+// kind and number of parts (17 to 10,000 tokens, 768 to 20,000 outputs over 768 to 14,336; several sets of weights in turn, which
+// the last-level cache still holds for 200 of the sizes), of which the choice is 0.7% behind the fastest on average, more than
+// 4.4% in one of 20 and 15% at worst (68 x 4,096 over 14,336; MI355X; profiles/int8_tile_times.txt).  It does not know whether
+// weights come from memory: 509 x 2,560 over 9,728 by 64 x 128 tiles 24.6 us from the last-level cache and 36 from memory, by
+// 128 x 128 in three parts 27 to 28 and 30.5.  Both sides of it, us, from the cache: 509 x 2,560 over 9,728 by 64 x 128 tiles
+// 24.6, 128 x 128 32.2, 64 x 64 30.8; 448 x 2,048 over 6,144 by 64 x 64 17.2, 64 x 128 23.8; 1,024 x
 // 6,144 over 2,560 by 128 x 256 25.4, 128 x 128 33, 256 x 256 36.5; 2,048 x 6,144 over 2,560 by 256 x 192 43.2, 256 x 256 46.5,
 // 128 x 256 52.8; 64 x 2,560 over 9,728 by 64 x 64 18.4, in 4 parts 13.5; 100 x 768 over 768 by 64 x 64 4.8, 256 x 256 14.9.
 inline I8Plan i8_plan(int M, int N, int K, bool gated, int cus) {
     // One tile of tokens over few outputs: 16 of them a block of 8 wavefronts, without LDS on the way (8 tokens x 2,560 over
     // 4,096 5.7 us, by 32 x 128 tiles 10.3; 16 x 2,560 over 9,728 11.2 and 12.2; but 8 x 9,728 gated over 2,560 14.9 and 13.6,
-    // 16 x 151,936 over 2,048 83 and 52).
+    // 16 x 151,936 over 2,048 83 and 52, where part of the weights comes from the last-level cache; all from memory 60).
     if (M <= 16 && (N + 15) / 16 * (gated ? 2 : 1) <= 2 * cus) return I8Plan{kRows, 1};
     I8Plan best{kTile256, 1};
     double least = 1e30;

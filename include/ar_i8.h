@@ -58,10 +58,13 @@ int ar_hip_embed_i8(ar_hip_ctx *ctx, const ar_rows_i8 *table, const int32_t *tok
  *   AR_GEMM_STORE:    C = p(W) (+ bias[n] where bias, fp32, is given)
  *   AR_GEMM_RESIDUAL: C += p(W)
  *   AR_GEMM_SWIGLU:   C = p(W2) * silu(p(W)): W the gate's rows, W2 the up projection's, of W's sizes and stride
- * C is of c_dtype (AR_DTYPE_F32 or AR_DTYPE_BF16), ldc values apart, N .. 2^24, rounded once.  A->rows * W->rows is at most 2^40.
+ * C is of c_dtype (AR_DTYPE_F32 or AR_DTYPE_BF16), ldc values apart, N .. 2^24.  A->rows * W->rows is at most 2^40.
+ * The sum goes to fp32 and each scale, the addition and the gate's steps round there; a bf16 result is rounded once more.
+ * Scales may be any finite numbers: what is computed on the way leaves fp32 only where a product, a gate or a result does.
  * Results do not depend on how a product is cut: the same rows give the same bits in any batch.
  * `work`: device memory of the caller's, 16-byte aligned, of at least the bytes that ar_hip_gemm_i8_work reports (null
- * where that is 0); its contents mean nothing between calls.  Calls ordered on one stream may share it, calls that may
+ * where that is 0) for these very sizes: it does not grow with them (2,560 outputs over 9,728: nothing for 16 tokens, 7.9 MB
+ * for 128, nothing for 509), so a caller with many sizes asks for each.  Its contents mean nothing between calls.  Calls ordered on one stream may share it, calls that may
  * run at the same time may not. */
 int ar_hip_gemm_i8_work(ar_hip_ctx *ctx, int M, int N, int K, int epilogue, size_t *bytes);
 int ar_hip_gemm_i8(ar_hip_ctx *ctx, const ar_rows_i8 *A, const ar_rows_i8 *W, const ar_rows_i8 *W2, const float *bias,
