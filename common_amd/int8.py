@@ -104,7 +104,7 @@ class Int8Ops:
         self.close()
 
     def _check_device(self, rows: Int8Rows):
-        if rows.ctx is not self.ctx and rows.ctx.index != self.ctx.index:
+        if rows.ctx not in (None, self.ctx) and rows.ctx.index != self.ctx.index:  # (None: on buffers of the caller's)
             raise ValueError(f"rows of device {rows.ctx.index} cannot be used on device {self.ctx.index}")
 
     def rows(self, rows: int, n: int) -> Int8Rows:

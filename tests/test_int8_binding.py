@@ -80,3 +80,12 @@ def test_rows_of_another_device_are_refused(call):
     assert len(ops.ctx.bufs) == 2  # (no work space was taken for it)
     with pytest.raises(hw.HardwareException, match="ctx is null"):
         CALLS[call](ops, rows, int8.Int8Rows(_Context(0), 8, 40))
+
+
+@pytest.mark.parametrize("call", sorted(CALLS))
+def test_rows_on_given_buffers_need_no_context(call):
+    """Rows made without one, on the caller's buffers, are used as before."""
+    ops = int8.Int8Ops(_Context(0))
+    rows, other = (int8.Int8Rows(None, 8, 40, q=_Buf(4096), scale=_Buf(8192)) for _ in range(2))
+    with pytest.raises(hw.HardwareException, match="ctx is null"):
+        CALLS[call](ops, rows, other)
